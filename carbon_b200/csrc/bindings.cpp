@@ -497,10 +497,12 @@ void indexer_topk(torch::Tensor q, torch::Tensor w, torch::Tensor kc, torch::Ten
 
 void register_runtime(pybind11::module_& m);
 void register_p2p(pybind11::module_& m);
+void register_tree(pybind11::module_& m);
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   register_runtime(m);
   register_p2p(m);
+  register_tree(m);
   m.doc() = "carbon_b200 sm_100a kernels";
   m.def("act_quant", &act_quant);
   m.def("rms_norm", &rms_norm);

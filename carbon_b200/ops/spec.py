@@ -1,0 +1,277 @@
+"""Speculative decoding over trees of drafted tokens: attention, verification and the commit of the accepted branch.
+
+One step runs, for every request, a small tree of drafted tokens (node 0 is the pending token, every other node
+continues its parent) through the model in one forward.  ``TreePlan`` holds the step's layout on the device; the three
+operators take it:
+
+* ``tree_mla``     absorbed MLA / latent-MQA attention of all nodes: each node sees its request's whole context and its
+                   own branch of the tree.  The cached rows are read once per 128 query rows (nodes x heads), not once
+                   per node (``sparse_mla`` gathers every row's key list again).
+* ``tree_verify``  the walk down the tree that accepts drafted tokens against the target's probabilities from given
+                   random numbers, and the token that follows (temperature 0: greedy agreement).
+* ``tree_commit``  the accepted nodes' cached rows, in every cache of a ``CacheRows``, moved behind the context.
+
+Conventions: the rows of a request's nodes are consecutive (``plan.cu``); node i of request b writes its cache rows at
+position ``ctx[b] + i`` of the request's page table.  Everything runs on the current stream, allocates from the caching
+allocator and neither waits for the device nor reads from it.  The oracle is ``ref.ops.tree_attention`` /
+``tree_verify``; CPU tensors use it.  The reference verifies chains of drafts as ordinary decode rows
+(``king_v10/bundle_v9/dec/gemm_tables.py:51``, ``dec/cuda_vattn.py:4654``).
+"""
+from __future__ import annotations
+
+from typing import List, NamedTuple, Optional, Sequence
+
+import torch
+
+from ..ref import ops as R
+from ._ext import ext
+
+MAX_NODES = 64           # nodes of one request's tree: one bit each in a node's mask
+
+
+class TreePlan:
+    """Layout of one tree step.  page_tables[b] lists request b's pages (at least ctx[b] + n_b positions), ctx[b] its
+    cached tokens, parents[b][i] the parent of node i (-1 for the root, node 0; parents come before children).
+    ``masks``: per request one integer per node, bit j = node i attends to node j; by default each node's ancestors
+    and itself.  Requests without nodes are allowed.  A plan serves every layer and operator of its step."""
+
+    def __init__(self, page_tables: Sequence[Sequence[int]], ctx: Sequence[int], parents: Sequence[Sequence[int]],
+                 page_size: int, n_heads: int = 1, device="cuda", masks: Optional[Sequence[Sequence[int]]] = None):
+        B = len(parents)
+        if len(page_tables) != B or len(ctx) != B or (masks is not None and len(masks) != B):
+            raise ValueError("TreePlan: page_tables, ctx, parents (and masks) need one entry per request")
+        if page_size < 1 or n_heads < 1:
+            raise ValueError("TreePlan: page_size and n_heads must be positive")
+        self.n = [len(p) for p in parents]
+        self.device = torch.device(device)
+        if self.device.type == "cuda" and self.device.index is None:
+            self.device = torch.device("cuda", torch.cuda.current_device())
+        self.page_size, self.n_heads = int(page_size), int(n_heads)
+        self.B, self.T, self.N = B, sum(self.n), max(self.n, default=0)
+        cu, req, par, pos, bits = [0], [], [], [], []
+        for b, (p, c, tab) in enumerate(zip(parents, ctx, page_tables)):
+            k = len(p)
+            if k > MAX_NODES:
+                raise ValueError(f"TreePlan: request {b} has {k} nodes, at most {MAX_NODES} are supported")
+            if c < 0 or (c + k + page_size - 1) // page_size > len(tab):
+                raise ValueError(f"TreePlan: request {b} has pages for {len(tab) * page_size} positions, its context "
+                                 f"and nodes need {c + k}")
+            if any(pg < 0 for pg in tab):
+                raise ValueError(f"TreePlan: request {b} has a negative page")
+            depth = []
+            for i, q in enumerate(p):
+                if not (q == -1 if i == 0 else 0 <= q < i):
+                    raise ValueError(f"TreePlan: request {b}: the parent of node {i} must be an earlier node "
+                                     "(-1 for node 0 only)")
+                depth.append(depth[q] + 1 if i else 0)
+            m = R.tree_masks(p) if masks is None else [int(x) for x in masks[b]]
+            if len(m) != k or any(x < 0 or x >> k for x in m):
+                raise ValueError(f"TreePlan: request {b} needs one mask of {k} bits per node")
+            bits += [x - (1 << 64) if x >> 63 else x for x in m]
+            cu.append(cu[-1] + k)
+            req += [b] * k
+            par += p
+            pos += [c + d for d in depth]
+        self.ctx_list, self.tables_list, self.parents_list = [int(c) for c in ctx], page_tables, parents
+        self.cu_list, self.pos_list = cu, pos
+        self.max_page = max((pg for tab in page_tables for pg in tab), default=-1)
+        P = max([len(t) for t in page_tables] + [1])
+        flat = []
+        for tab in page_tables:
+            flat += list(tab)
+            flat += [0] * (P - len(tab))
+        # one host buffer, one copy: masks (64 bits) first, then the 32-bit lists
+        T = self.T
+        words = torch.tensor(bits, dtype=torch.int64).view(torch.int32)
+        ints = torch.tensor(cu + list(ctx) + req + par + pos + flat, dtype=torch.int32)
+        host = torch.cat([words, ints])
+        if self.device.type == "cuda":
+            host = host.pin_memory()
+        dev = host.to(self.device, non_blocking=True)
+        self.mask = dev[:2 * T].view(torch.int64)
+        at = 2 * T
+        out = []
+        for k in (B + 1, B, T, T, T, B * P):
+            out.append(dev[at:at + k])
+            at += k
+        self.cu, self.ctx, self.req, self.parent, self.pos, self.table = out
+        self.table = self.table.view(B, P)
+
+    def slots(self, b: int, n: Optional[int] = None) -> List[int]:
+        """Cache slots of request b's first n positions (default: its context and all its nodes)."""
+        ps, tab = self.page_size, self.tables_list[b]
+        n = self.ctx_list[b] + self.n[b] if n is None else n
+        return [tab[i // ps] * ps + i % ps for i in range(n)]
+
+    def node_slots(self) -> List[int]:
+        """Cache slot of every node row."""
+        ps = self.page_size
+        return [tab[(c + i) // ps] * ps + (c + i) % ps
+                for tab, c, k in zip(self.tables_list, self.ctx_list, self.n) for i in range(k)]
+
+    def _check(self, what: str, slots: int):
+        if (self.max_page + 1) * self.page_size > slots:
+            raise ValueError(f"{what}: the plan's pages reach slot {(self.max_page + 1) * self.page_size - 1}, the "
+                             f"cache holds {slots}")
+
+
+def _need(what: str, t: torch.Tensor, device, dtype) -> None:
+    if t.dtype != dtype or t.device != device or not t.is_contiguous():
+        raise ValueError(f"{what} must be contiguous {dtype} on {device}, got {t.dtype} on {t.device}"
+                         f"{'' if t.is_contiguous() else ' (not contiguous)'}")
+
+
+def _launched(code: int, what: str) -> None:
+    if code:
+        raise RuntimeError(f"{what}: CUDA error {code} at launch")
+
+
+def tree_mla(q: torch.Tensor, kv: torch.Tensor, plan: TreePlan, scale: float, d_latent: int = 512,
+             sink: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention of the plan's nodes over the paged latent cache: q [T, H, D], kv [S, D] bf16 (or the fp8 cache rows,
+    uint8 [S, row_bytes], with q in fp16; q is converted), D = 576 (MLA) or 512 (latent MQA) -> [T, H, 512] bf16.
+    sink [H]: per-head attention-sink logit.  A node that sees no key gives zeros."""
+    T, H, D = q.shape
+    f8 = kv.dtype == torch.uint8
+    if T != plan.T:
+        raise ValueError(f"tree_mla: q has {T} rows, the plan {plan.T} nodes")
+    plan._check("tree_mla", kv.shape[0])
+    if sink is not None and tuple(sink.shape) != (H,):
+        raise ValueError(f"tree_mla: sink has shape {tuple(sink.shape)}, expected {(H,)}")
+    if q.is_cuda:
+        if D not in (576, 512) or d_latent != 512:
+            raise RuntimeError("tree_mla: the kernel needs D=576 (512 latent + 64 RoPE key) or D=512 (latent MQA) and "
+                               "d_latent=512")
+        if H != plan.n_heads:
+            raise ValueError(f"tree_mla: q has {H} heads, the plan was made for {plan.n_heads}")
+        if q.device != plan.device:
+            raise ValueError(f"tree_mla: q is on {q.device}, the plan on {plan.device}")
+        _need("tree_mla: kv", kv, q.device, torch.uint8 if f8 else torch.bfloat16)
+        if kv.dim() != 2 or kv.shape[1] != (R.latent_fp8_row_bytes(512, 64, D == 576) if f8 else D):
+            raise ValueError(f"tree_mla: kv of shape {tuple(kv.shape)} does not hold rows for width {D}")
+        qk = q.to(torch.float16 if f8 else torch.bfloat16).contiguous()
+        if sink is not None:
+            sink = sink.to(q.device, torch.float32).contiguous()
+        out = torch.empty(T, H, 512, dtype=torch.bfloat16, device=q.device)
+        if T:
+            _launched(ext().tree_mla(qk, kv, plan.cu, plan.ctx, plan.table, plan.mask, plan.req, plan.page_size,
+                                     float(scale), sink, out), "tree_mla")
+        return out
+    out = torch.zeros(T, H, d_latent)
+    mla = D > d_latent
+    for b in range(plan.B):
+        lo, hi = plan.cu_list[b], plan.cu_list[b + 1]
+        rows = kv[torch.tensor(plan.slots(b), dtype=torch.long)]
+        rows = R.dequant_latent_fp8(rows, d_latent, D - d_latent if mla else 0, mla) if f8 else rows.float()
+        out[lo:hi] = R.tree_attention(q[lo:hi].float(), rows, plan.ctx_list[b], plan.mask[lo:hi].tolist(), scale,
+                                      d_latent, sink)
+    return out
+
+
+class TreeVerdict(NamedTuple):
+    """Outcome of ``tree_verify``, N = the largest tree's nodes: path [B, N] the accepted nodes (the root first),
+    n_accepted [B] how many drafted nodes were accepted, tokens [B, N] the accepted tokens and then the next one,
+    logprobs [B, N] their log-probabilities under the target at the request's temperature (at 1 when greedy).
+    path and tokens are padded with -1, logprobs with 0.  A request without nodes has n_accepted -1."""
+
+    path: torch.Tensor
+    n_accepted: torch.Tensor
+    tokens: torch.Tensor
+    logprobs: torch.Tensor
+
+
+def tree_verify(logits: torch.Tensor, tokens: torch.Tensor, plan: TreePlan, uniforms: torch.Tensor,
+                noise: torch.Tensor, temperature: torch.Tensor, draft_probs: Optional[torch.Tensor] = None
+                ) -> TreeVerdict:
+    """Accept or reject the drafted tokens (``ref.ops.tree_verify`` states the rule).  logits [T, V] fp32 or bf16 (unit
+    column stride): the target's logits at every node; tokens [T] int32: every node's token (the root's is not
+    tested); uniforms [T] fp32 in [0, 1): one per node; noise [B, V] fp32: Exp(1) variates; temperature [B] fp32 (0 =
+    greedy); draft_probs [T, V] fp32: row t = the distribution that node t's children were drawn from (independent
+    draws), None = certain proposals (prompt lookup, a draft model's best tokens).  The emitted tokens are distributed
+    as the target's own samples."""
+    T, B, V = plan.T, plan.B, logits.shape[1]
+    for name, t, shape in (("logits", logits, (T, V)), ("tokens", tokens, (T,)), ("uniforms", uniforms, (T,)),
+                           ("noise", noise, (B, V)), ("temperature", temperature, (B,)),
+                           ("draft_probs", draft_probs, (T, V))):
+        if t is not None and tuple(t.shape) != shape:
+            raise ValueError(f"tree_verify: {name} has shape {tuple(t.shape)}, expected {shape}")
+    N = plan.N
+    if logits.is_cuda:
+        dev = plan.device
+        if logits.device != dev or logits.dtype not in (torch.float32, torch.bfloat16) or not 0 < V < 1 << 31 or (
+                T and logits.stride(1) != 1):
+            raise ValueError(f"tree_verify: logits must be fp32 or bf16 on {dev} with a unit column stride, got "
+                             f"{logits.dtype} on {logits.device}, strides {logits.stride()}")
+        _need("tree_verify: tokens", tokens, dev, torch.int32)
+        _need("tree_verify: uniforms", uniforms, dev, torch.float32)
+        _need("tree_verify: noise", noise, dev, torch.float32)
+        _need("tree_verify: temperature", temperature, dev, torch.float32)
+        if draft_probs is not None:
+            _need("tree_verify: draft_probs", draft_probs, dev, torch.float32)
+        out = torch.empty(B * (2 * N + 1), dtype=torch.int32, device=dev)
+        lp = torch.empty(B, N, dtype=torch.float32, device=dev)
+        if B:
+            _launched(ext().tree_verify(logits, tokens, plan.cu, plan.parent, N, uniforms, noise, temperature,
+                                        draft_probs, out, lp), "tree_verify")
+        return TreeVerdict(out[:B * N].view(B, N), out[2 * B * N:], out[B * N:2 * B * N].view(B, N), lp)
+    v = TreeVerdict(torch.full((B, N), -1, dtype=torch.int32), torch.full((B,), -1, dtype=torch.int32),
+                    torch.full((B, N), -1, dtype=torch.int32), torch.zeros(B, N))
+    for b in range(B):
+        lo, hi = plan.cu_list[b], plan.cu_list[b + 1]
+        if lo == hi:
+            continue
+        path, toks, lps = R.tree_verify(logits[lo:hi].float(), tokens[lo:hi], plan.parents_list[b], uniforms[lo:hi],
+                                        noise[b], float(temperature[b]),
+                                        draft_probs[lo:hi] if draft_probs is not None else None)
+        v.path[b, :len(path)] = torch.tensor(path, dtype=torch.int32)
+        v.tokens[b, :len(toks)] = torch.tensor(toks, dtype=torch.int32)
+        v.logprobs[b, :len(lps)] = torch.tensor(lps)
+        v.n_accepted[b] = len(path) - 1
+    return v
+
+
+class CacheRows:
+    """The caches whose rows move together: tensors [S, ...] (one row per slot, any row size that is a multiple of 4
+    bytes), contiguous and on one device.  Holds the tensors and, on a GPU, the table of their addresses."""
+
+    def __init__(self, caches: Sequence[torch.Tensor]):
+        self.caches = [c for c in caches if c is not None]
+        if not self.caches:
+            raise ValueError("CacheRows: no caches")
+        first = self.caches[0]
+        self.device = first.device
+        self.slots = min(c.shape[0] for c in self.caches)
+        rows = []
+        for c in self.caches:
+            nbytes = c[0].numel() * c.element_size() if c.shape[0] else 0
+            if c.device != first.device or not c.is_contiguous() or nbytes % 4 or not nbytes:
+                raise ValueError("CacheRows: caches must be contiguous, on one device and have rows of a multiple of "
+                                 "4 bytes")
+            rows += [c.data_ptr(), nbytes]
+        self.max_row = max(rows[1::2])
+        self.wide = all(x % 16 == 0 for x in rows)
+        self.table = torch.tensor(rows, dtype=torch.int64).view(-1, 2).to(first.device)
+
+
+def tree_commit(rows: CacheRows, plan: TreePlan, path: torch.Tensor, n_accepted: torch.Tensor) -> None:
+    """Move the accepted branch's cache rows behind the context, in place: for k = 1 .. n_accepted[b], the row of node
+    path[b, k] goes to position ctx[b] + k (node k's old row).  path [B, N] and n_accepted [B] as ``tree_verify``
+    returns them."""
+    if tuple(path.shape) != (plan.B, plan.N) or tuple(n_accepted.shape) != (plan.B,):
+        raise ValueError(f"tree_commit: path {tuple(path.shape)} and n_accepted {tuple(n_accepted.shape)}, expected "
+                         f"{(plan.B, plan.N)} and {(plan.B,)}")
+    plan._check("tree_commit", rows.slots)
+    if rows.device.type == "cuda":
+        if rows.device != plan.device:
+            raise ValueError(f"tree_commit: the caches are on {rows.device}, the plan on {plan.device}")
+        _need("tree_commit: path", path, rows.device, torch.int32)
+        _need("tree_commit: n_accepted", n_accepted, rows.device, torch.int32)
+        if plan.N > 1:
+            _launched(ext().tree_commit(rows.table, rows.max_row, rows.wide, plan.cu, plan.ctx, plan.table,
+                                        plan.page_size, path, n_accepted), "tree_commit")
+        return
+    for b in range(plan.B):
+        s = plan.slots(b)[plan.ctx_list[b]:]
+        for k in range(1, int(n_accepted[b]) + 1):
+            for c in rows.caches:
+                c[s[k]] = c[s[int(path[b, k])]]

@@ -456,3 +456,86 @@ def engram_gate(X: torch.Tensor, kv: torch.Tensor, q_w: torch.Tensor, k_w: torch
     s = (xn * kn).sum(-1) / math.sqrt(D)
     g = torch.sigmoid(s.clamp(-clamp, clamp))                                  # [T, hc]
     return Xf + g[..., None] * v[:, None, :]
+
+
+# ----------------------------------------------------------------------------------------------------------------------
+# speculative decoding over a tree of drafted tokens
+# ----------------------------------------------------------------------------------------------------------------------
+def tree_masks(parents) -> list:
+    """Ancestor bit masks of one request's tree: bit j of entry i is set when node i attends to node j (itself and
+    the nodes between it and the root).  ``parents[i] < i`` is the parent's index, -1 for a root."""
+    out = []
+    for i, p in enumerate(parents):
+        out.append((1 << i) | (out[p] if p >= 0 else 0))
+    return out
+
+
+def tree_attention(q: torch.Tensor, keys: torch.Tensor, ctx: int, masks, scale: float, r: int,
+                   sink: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """One request's drafted nodes over its latent rows: q [n, H, D], keys [ctx + n, D] (node i's row at ctx + i).
+    Node i attends to every key before ctx and to the nodes whose bit is set in masks[i]; the value of a key is its
+    first r dims.  A node that sees nothing gives zeros.  Computed in q's precision."""
+    n, H = q.shape[0], q.shape[1]
+    out = torch.zeros(n, H, r, dtype=q.dtype, device=q.device)
+    for i in range(n):
+        sel = list(range(ctx)) + [ctx + j for j in range(n) if int(masks[i]) >> j & 1]
+        if not sel:
+            continue
+        k = keys[sel]
+        s = q[i] @ k.t() * scale
+        if sink is not None:
+            s = torch.cat([s, sink.to(s.dtype)[:, None]], -1)
+        out[i] = torch.softmax(s, -1)[:, :len(sel)] @ k[:, :r]
+    return out
+
+
+def tree_verify(logits: torch.Tensor, tokens, parents, uniforms, noise: torch.Tensor, temperature: float,
+                draft_probs: Optional[torch.Tensor] = None):
+    """Walk of one request's drafted tree against the target (speculative sampling with several candidates per
+    node): at node v with target probabilities r = softmax(logits[v] / T), each child c in index order is accepted
+    when u_c q(x_c) < r(x_c), q the distribution its token was drawn from (draft_probs[v]; without them the token is
+    a certain proposal, q = 1 at it); a rejection leaves r <- max(r - q, 0) renormalised (r itself if nothing is
+    left).  Where no child is accepted the next token is argmax_i r_i / noise_i (noise ~ Exp(1): a draw from r; ties
+    to the lowest index).  T <= 0: r is one at the lowest-index maximum of the logits and no noise is used.
+    Returns (path, tokens, logprobs): the accepted nodes from the root, the emitted tokens (-1 if r has no mass) and
+    their log-probabilities under softmax(logits / T) (T = 1 when greedy)."""
+    heat = temperature if temperature > 0 else 1.0
+    v, path, toks, lps = 0, [0], [], []
+    while True:
+        lp = torch.log_softmax(logits[v] / heat, -1)
+        if bool(torch.isneginf(logits[v]).all()):
+            r = torch.zeros_like(lp)
+            lp = torch.full_like(lp, float("-inf"))
+        elif temperature > 0:
+            r = lp.exp()
+        else:
+            r = torch.zeros_like(lp)
+            r[int(torch.argmax((logits[v] == logits[v].max()).int()))] = 1.0
+        nxt = -1
+        for c in [j for j in range(len(parents)) if parents[j] == v]:
+            x = int(tokens[c])
+            q = torch.zeros_like(r)
+            if draft_probs is None:
+                q[x] = 1.0
+                rest = r.clone()
+                rest[x] = 0.0
+            else:
+                q = draft_probs[v].to(r.dtype)
+                rest = (r - q).clamp(min=0)
+            if float(uniforms[c]) * float(q[x]) < float(r[x]):
+                nxt = c
+                break
+            if float(rest.sum()) > 0:
+                r = rest / rest.sum()
+        if nxt < 0:
+            break
+        toks.append(x)
+        lps.append(float(lp[x]))
+        path.append(nxt)
+        v = nxt
+    score = torch.where(r > 0, r / noise.to(r.dtype) if temperature > 0 else r, -torch.ones_like(r))
+    best = int(torch.argmax((score == score.max()).int()))
+    ok = float(score[best]) > 0
+    toks.append(best if ok else -1)
+    lps.append(float(lp[best]) if ok else float("-inf"))
+    return path, toks, lps
