@@ -4,6 +4,11 @@
 #include <torch/extension.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
+#include <algorithm>
+#include <cstring>
+#include <queue>
+#include <tuple>
+#include <vector>
 #include "tree.h"
 
 namespace {
@@ -22,13 +27,122 @@ cb::TreeLayout layout(const Tensor& cu, const Tensor& ctx, const Tensor& table, 
   return {ptr<int>(cu), ptr<int>(ctx), ptr<int>(table), int(table.size(0)), int(table.size(1)), int(page)};
 }
 
+// Split of one attention call over `clusters` CTA pairs (csrc/tree.h: TreeWork).  Every row tile of every request is a
+// list of ceil((ctx + n) / 128) key tiles; longest first, each goes to the pair with the least work so far, and where it
+// would pass the even share it is cut there and the rest goes on to the next pair (partial results are merged).  The
+// row tiles of a request are handed out one after the other, so they run at about the same time and read its keys from
+// L2.  kOver: cost of an item's start and end in key tiles.
+// -> int32 tensor: first [clusters + 1], items [*, 5], merges [*, 4], (even offset) staged blocks of the tail mode
+// [*, 2], of the all mode [*, 2], first block per request of either [B] [B]; and the counts
+std::tuple<Tensor, std::vector<int64_t>> tree_schedule(const std::vector<int64_t>& n, const std::vector<int64_t>& ctx,
+                                                       int64_t H, int64_t clusters) {
+  constexpr int64_t kTile = 128, kOver = 2;
+  const int64_t B = int64_t(n.size());
+  struct Row { int64_t b, row, tiles; };
+  std::vector<Row> rows;
+  int64_t total = 0;
+  for (int64_t b = 0; b < B; ++b) {
+    const int64_t tiles = (ctx[b] + n[b] + kTile - 1) / kTile;
+    for (int64_t r = 0; r < (n[b] * H + 127) / 128; ++r, total += tiles + kOver) rows.push_back({b, r, tiles});
+  }
+  std::stable_sort(rows.begin(), rows.end(), [](const Row& x, const Row& y) { return x.tiles > y.tiles; });
+  clusters = std::max<int64_t>(1, clusters);
+  const int64_t share = (total + clusters - 1) / clusters;
+  using Load = std::pair<int64_t, int64_t>;                       // (work, pair)
+  std::priority_queue<Load, std::vector<Load>, std::greater<Load>> heap;
+  for (int64_t c = 0; c < clusters; ++c) heap.push({0, c});
+  std::vector<std::vector<cb::TreeItem>> lists(clusters);
+  std::vector<cb::TreeMerge> merges;
+  int64_t parts = 0;
+  for (const Row& r : rows) {
+    int64_t at = 0;
+    const int64_t first_part = parts;
+    std::vector<std::pair<int64_t, size_t>> pieces;
+    while (at < r.tiles) {
+      const Load ld = heap.top();
+      heap.pop();
+      const int64_t rest = r.tiles - at, room = std::max<int64_t>(1, share - ld.first - kOver);
+      const int64_t take = rest <= room + 1 ? rest : room;
+      auto& list = lists[ld.second];
+      pieces.push_back({ld.second, list.size()});
+      list.push_back({int(r.b), int(r.row), int(at), int(take), -1});
+      heap.push({ld.first + take + kOver, ld.second});
+      at += take;
+    }
+    if (pieces.size() > 1) {
+      for (auto& [c, i] : pieces) lists[c][i].part = int(parts++);
+      merges.push_back({int(r.b), int(r.row), int(first_part), int(pieces.size())});
+    }
+  }
+  int64_t used = 0, n_items = 0, n_tail = 0, n_all = 0;
+  for (auto& l : lists) { used += !l.empty(); n_items += int64_t(l.size()); }
+  std::stable_sort(lists.begin(), lists.end(), [](const auto& x, const auto& y) { return !x.empty() && y.empty(); });
+  for (int64_t b = 0; b < B; ++b) {
+    if (!n[b]) continue;
+    const int64_t tiles = (ctx[b] + n[b] + kTile - 1) / kTile;
+    n_tail += tiles - ctx[b] / kTile;
+    n_all += tiles;
+  }
+  int64_t size = used + 1 + n_items * 5 + int64_t(merges.size()) * 4;
+  size += size & 1;
+  auto out = torch::empty({size + 2 * n_tail + 2 * n_all + 2 * B}, torch::kInt32);
+  int* o = ptr<int>(out);
+  int* items = o + used + 1;
+  o[0] = 0;
+  int at = 0;
+  for (int64_t c = 0; c < used; ++c) {
+    for (const auto& it : lists[c]) std::memcpy(items + 5 * at++, &it, sizeof it);
+    o[c + 1] = at;
+  }
+  if (!merges.empty()) std::memcpy(items + 5 * n_items, merges.data(), merges.size() * sizeof merges[0]);
+  int* tail = o + size;
+  int* all = tail + 2 * n_tail;
+  int* at_tail = all + 2 * n_all;
+  int* at_all = at_tail + B;
+  int it = 0, ia = 0;
+  for (int64_t b = 0; b < B; ++b) {
+    at_tail[b] = it;
+    at_all[b] = ia;
+    if (!n[b]) continue;
+    const int64_t tiles = (ctx[b] + n[b] + kTile - 1) / kTile;
+    for (int64_t t = 0; t < tiles; ++t) {
+      all[2 * ia] = int(b);
+      all[2 * ia++ + 1] = int(t);
+      if (t < ctx[b] / kTile) continue;
+      tail[2 * it] = int(b);
+      tail[2 * it++ + 1] = int(t);
+    }
+  }
+  return {out, {used, n_items, int64_t(merges.size()), parts, n_tail, n_all, size}};
+}
+
+// work: tree_schedule's tensor on the device, counts its counts; buf: workspace (sizes in tree_mla_workspace's order:
+// staged rows, bad [T], partial outputs, partial (m, l)) at byte offsets off[0..3]
 int tree_mla(const Tensor& q, const Tensor& kv, const Tensor& cu, const Tensor& ctx, const Tensor& table,
-             const Tensor& mask, const Tensor& req, int64_t page, double scale, const OptTensor& sink,
-             const Tensor& out) {
+             const Tensor& mask, int64_t page, bool all, const Tensor& work, const std::vector<int64_t>& counts,
+             const Tensor& buf, const std::vector<int64_t>& off, double scale, const OptTensor& sink,
+             const Tensor& status, const Tensor& out) {
   c10::cuda::CUDAGuard g(q.device());
-  return cb::tree_mla(q.data_ptr(), q.size(0), q.size(1), q.size(2), kv.scalar_type() == at::kByte, kv.data_ptr(),
-                      layout(cu, ctx, table, page), ptr<int64_t>(mask), ptr<int>(req), float(scale), ptr<float>(sink),
-                      out.data_ptr(), stream());
+  const int64_t used = counts[0], n_items = counts[1], n_merges = counts[2], n_tail = counts[4], n_all = counts[5];
+  const int* w = ptr<int>(work);
+  const int* tail = w + counts[6];
+  const int* every = tail + 2 * n_tail;
+  const int* at = every + 2 * n_all;
+  cb::TreeWork tw;
+  tw.first = w;
+  tw.items = reinterpret_cast<const cb::TreeItem*>(w + used + 1);
+  tw.merges = reinterpret_cast<const cb::TreeMerge*>(w + used + 1 + 5 * n_items);
+  tw.clusters = int(used);
+  tw.n_merges = int(n_merges);
+  tw.n_parts = int(counts[3]);
+  tw.stage = reinterpret_cast<const int2*>(all ? every : tail);
+  tw.stage_at = at + (all ? table.size(0) : 0);
+  tw.n_stage = int(all ? n_all : n_tail);
+  uint8_t* ws = ptr<uint8_t>(buf);
+  return cb::tree_mla(q.data_ptr(), q.size(0), q.size(1), q.size(2), kv.scalar_type() == at::kByte, all, kv.data_ptr(),
+                      kv.size(0), layout(cu, ctx, table, page), tw, ptr<int64_t>(mask), float(scale), ptr<float>(sink),
+                      ws + off[0], reinterpret_cast<int*>(ws + off[1]), reinterpret_cast<float*>(ws + off[2]),
+                      reinterpret_cast<float*>(ws + off[3]), ptr<int>(status), out.data_ptr(), stream());
 }
 
 // out: int32 [B (2 N + 1)] = path, tokens, n_accepted
@@ -54,6 +168,8 @@ int tree_commit(const Tensor& caches, int64_t max_row, bool wide, const Tensor& 
 }  // namespace
 
 void register_tree(pybind11::module_& m) {
+  m.def("tree_schedule", &tree_schedule);
+  m.def("tree_mla_clusters", [] { return cb::tree_mla_clusters(); });
   m.def("tree_mla", &tree_mla);
   m.def("tree_verify", &tree_verify);
   m.def("tree_commit", &tree_commit);

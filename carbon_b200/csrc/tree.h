@@ -14,10 +14,30 @@ struct TreeLayout {
   int B, P, page;
 };
 
+// Work of one attention call, made by tree_schedule: a CTA pair runs the items [first[c], first[c + 1]) one after the
+// other.  An item is one 128-row tile (rows = nodes x heads of one request) over a range of 128-key tiles.
+struct TreeItem { int b, row, tile, n_tiles, part; };      // part: partial-result slot, -1 = the whole row tile
+struct TreeMerge { int b, row, part, n; };                 // row tile whose partial results [part, part + n) are merged
+struct TreeWork {
+  const int* first;        // [clusters + 1]
+  const TreeItem* items;
+  const TreeMerge* merges;
+  int clusters, n_merges, n_parts;
+  // 128-row blocks of the staging buffer: (request, key tile) each; the request's first block is stage_at[b] and its
+  // first staged key tile stage_tile(b): 0 when every row is staged, else ctx / 128
+  const int2* stage;
+  const int* stage_at;     // [B]
+  int n_stage;
+};
+
 // q [T, H, D] (bf16; fp16 for fp8 rows), kv rows [S, row bytes], mask [T] (bit j: the node sees node j), req [T]
-// -> out [T, H, 512] bf16
-cudaError_t tree_mla(const void* q, int T, int H, int D, bool f8, const void* kv, const TreeLayout& lay,
-                     const int64_t* mask, const int* req, float scale, const float* sink, void* out, cudaStream_t s);
+// -> out [T, H, 512] bf16.  all: every key row is staged (fp8 rows; pages that are no multiple of 8).
+// staged [n_stage * 128, D] 16-bit, bad [T], part_o [n_parts, 128, 512], part_ml [n_parts, 128, 2]: workspaces.
+cudaError_t tree_mla(const void* q, int T, int H, int D, bool f8, bool all, const void* kv, int64_t S,
+                     const TreeLayout& lay, const TreeWork& work, const int64_t* mask, float scale, const float* sink,
+                     void* staged, int* bad, float* part_o, float* part_ml, int* status, void* out, cudaStream_t s);
+// CTA pairs of the attention kernel that fit on the current device at once
+int tree_mla_clusters();
 
 // logits [T, ld] fp32 or bf16, draft [T, V] fp32 or null -> path, tokens [B, N], n_accepted [B], logprobs [B, N]
 cudaError_t tree_verify(const void* logits, bool bf16, int64_t ld, int V, const int* tokens, const int* cu,

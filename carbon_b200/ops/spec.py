@@ -29,6 +29,19 @@ from ._ext import ext
 MAX_NODES = 64           # nodes of one request's tree: one bit each in a node's mask
 
 
+_CLUSTERS = {}
+
+
+def _clusters(device: torch.device) -> int:
+    """CTA pairs of the attention kernel that the device runs at once."""
+    if device not in _CLUSTERS:
+        with torch.cuda.device(device):
+            _CLUSTERS[device] = ext().tree_mla_clusters()
+        if not _CLUSTERS[device]:
+            raise RuntimeError(f"tree_mla: the attention kernel does not fit on {device}")
+    return _CLUSTERS[device]
+
+
 class TreePlan:
     """Layout of one tree step.  page_tables[b] lists request b's pages (at least ctx[b] + n_b positions), ctx[b] its
     cached tokens, parents[b][i] the parent of node i (-1 for the root, node 0; parents come before children).
@@ -80,22 +93,33 @@ class TreePlan:
         for tab in page_tables:
             flat += list(tab)
             flat += [0] * (P - len(tab))
-        # one host buffer, one copy: masks (64 bits) first, then the 32-bit lists
+        # one host buffer, one copy: masks (64 bits) first, the attention's work (64-bit aligned), the 32-bit lists
         T = self.T
         words = torch.tensor(bits, dtype=torch.int64).view(torch.int32)
-        ints = torch.tensor(cu + list(ctx) + req + par + pos + flat, dtype=torch.int32)
-        host = torch.cat([words, ints])
+        work, self._counts = torch.zeros(0, dtype=torch.int32), []
+        if self.device.type == "cuda" and T:
+            work, self._counts = ext().tree_schedule(self.n, [int(c) for c in ctx], self.n_heads,
+                                                     _clusters(self.device))
+        ints = torch.tensor(cu + list(ctx) + req + par + pos + flat + [0], dtype=torch.int32)
+        host = torch.cat([words, work, ints])
         if self.device.type == "cuda":
             host = host.pin_memory()
         dev = host.to(self.device, non_blocking=True)
         self.mask = dev[:2 * T].view(torch.int64)
-        at = 2 * T
+        self._work = dev[2 * T:2 * T + work.numel()]
+        self.status = dev[-1:]              # error code of a device-side wait that ran out (0: none)
+        at = 2 * T + work.numel()
         out = []
         for k in (B + 1, B, T, T, T, B * P):
             out.append(dev[at:at + k])
             at += k
         self.cu, self.ctx, self.req, self.parent, self.pos, self.table = out
         self.table = self.table.view(B, P)
+
+    def check(self) -> None:
+        """Raise if a kernel of this plan gave up a wait (reads from the device)."""
+        if int(self.status):
+            raise RuntimeError(f"tree_mla: device status {int(self.status)}: a bounded wait ran out")
 
     def slots(self, b: int, n: Optional[int] = None) -> List[int]:
         """Cache slots of request b's first n positions (default: its context and all its nodes)."""
@@ -136,6 +160,8 @@ def tree_mla(q: torch.Tensor, kv: torch.Tensor, plan: TreePlan, scale: float, d_
     if T != plan.T:
         raise ValueError(f"tree_mla: q has {T} rows, the plan {plan.T} nodes")
     plan._check("tree_mla", kv.shape[0])
+    if not scale > 0:
+        raise ValueError(f"tree_mla: scale must be positive, got {scale}")
     if sink is not None and tuple(sink.shape) != (H,):
         raise ValueError(f"tree_mla: sink has shape {tuple(sink.shape)}, expected {(H,)}")
     if q.is_cuda:
@@ -154,8 +180,19 @@ def tree_mla(q: torch.Tensor, kv: torch.Tensor, plan: TreePlan, scale: float, d_
             sink = sink.to(q.device, torch.float32).contiguous()
         out = torch.empty(T, H, 512, dtype=torch.bfloat16, device=q.device)
         if T:
-            _launched(ext().tree_mla(qk, kv, plan.cu, plan.ctx, plan.table, plan.mask, plan.req, plan.page_size,
-                                     float(scale), sink, out), "tree_mla")
+            # rows that TMA cannot take from the cache as they lie are staged: fp8 rows, pages that are no multiple of
+            # 8 rows (a swizzle group); else only each request's last tiles
+            whole = f8 or plan.page_size % 8 != 0
+            parts = plan._counts[3]
+            sizes = (plan._counts[5 if whole else 4] * 256 * D, 4 * T, parts * 128 * 2048, parts * 128 * 8)
+            off, end = [], 0
+            for k in sizes:
+                off.append(end)
+                end += (k + 255) // 256 * 256
+            buf = torch.empty(end, dtype=torch.uint8, device=q.device)
+            _launched(ext().tree_mla(qk, kv, plan.cu, plan.ctx, plan.table, plan.mask, plan.page_size, whole,
+                                     plan._work, plan._counts, buf, off, float(scale), sink, plan.status, out),
+                      "tree_mla")
         return out
     out = torch.zeros(T, H, d_latent)
     mla = D > d_latent
