@@ -25,7 +25,10 @@ constexpr int SLOTS = 9;                   // chunks of a stage: the CTA's 64 ke
 constexpr int STAGE = SLOTS * CH;
 constexpr int NST = 2;
 constexpr int TM_O = 0, TM_S = 256;        // TMEM columns: O 256, two score buffers of 64
-constexpr int SMEM = 1024 + SLOTS * CH + NST * STAGE + CH + 3 * 512 + 256;
+constexpr int SM_WARPS = 8;                // softmax warps: two per 32 TMEM lanes, each one half of the score columns
+constexpr int THREADS = 128 + SM_WARPS * 32;
+constexpr int SMEM_USED = SLOTS * CH + NST * STAGE + CH + 2048 + 256;
+constexpr int SMEM = SMEM_USED + 768;      // 227 KB; the base is 256-byte aligned at least (checked by the kernel)
 constexpr float kRescale = 8.f;            // O is rescaled when the running maximum grows by more than 2^8
 
 struct Params {
@@ -59,7 +62,7 @@ CB_DEVICE uint32_t pack2(float a, float b, bool f16) {
   }
   return pack_bf16x2(a, b);
 }
-CB_DEVICE void softmax_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
+CB_DEVICE void softmax_sync() { asm volatile("bar.sync 1, %0;" ::"n"(SM_WARPS * 32) : "memory"); }
 
 // ---------------------------------------------------------------------------------------------------------------
 // Rows [tile * 128, ...) of a request -> block of the staging buffer, zeros past its last node.  fp8 rows are expanded
@@ -148,19 +151,24 @@ __global__ void __launch_bounds__(256) tree_stage_kernel(const uint8_t* __restri
 // 64-127 into one extra chunk.
 //   producer (each CTA)  K(0) K(1) V(0) V(1) | K(2) K(3) V(2) V(3) | ...
 //   MMA (CTA 0)          QK(0) QK(1) PV(0) PV(1) | QK(2) QK(3) PV(2) PV(3) | ...
-//   softmax (each CTA)   thread = (row, half of the keys); the two threads of a row exchange their maxima
+//   softmax (each CTA)   thread = (row, 32 of the 128 keys); the four threads of a row exchange their maxima
 // ---------------------------------------------------------------------------------------------------------------
+// The tensor maps see a row as 64-dim atoms: (64 dims, rows, atoms), so one TMA load fills several chunks.
+struct Maps {
+  CUtensorMap q;            // box 64 x 64 rows x all atoms
+  CUtensorMap kv4, kv1;     // cache rows: box 64 x Params::box rows x 4 atoms / 1 atom (the RoPE key)
+  CUtensorMap st4, st1;     // staged rows: 64 rows
+};
+
 template <int NA, bool F16>
-__global__ void __launch_bounds__(256, 1) tree_mla_kernel(const __grid_constant__ CUtensorMap tm_q,
-                                                          const __grid_constant__ CUtensorMap tm_kv,
-                                                          const __grid_constant__ CUtensorMap tm_st, const Params p) {
+__global__ void __launch_bounds__(THREADS, 1) tree_mla_kernel(const __grid_constant__ Maps tm, const Params p) {
 #if defined(__CUDA_ARCH__) && __CUDA_ARCH__ >= 1000
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* sQ = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sK = sQ + SLOTS * CH;
   uint8_t* sX = sK + NST * STAGE;                       // P, keys 64-127
-  float* xm = reinterpret_cast<float*>(sX + CH);        // [2][128] row maxima, [128] row sums
-  uint64_t* bars = reinterpret_cast<uint64_t*>(xm + 384);
+  float* xm = reinterpret_cast<float*>(sX + CH);        // [2][256] row maxima (the last tile's buffer, later, sums)
+  uint64_t* bars = reinterpret_cast<uint64_t*>(xm + 512);
   uint64_t* q_full = bars;                              // the leader's counts both CTAs' bytes (so do kfull, vfull)
   uint64_t* o_free = bars + 1;                          // leader: both CTAs read the last item's O
   uint64_t* kfull = bars + 2;                           // [NST]
@@ -173,16 +181,20 @@ __global__ void __launch_bounds__(256, 1) tree_mla_kernel(const __grid_constant_
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(pv1 + NST);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
+  if (sQ + SMEM_USED > smem_raw + SMEM) {                // the same in every CTA
+    if (threadIdx.x == 0 && p.status) atomicCAS(p.status, 0, kErrBadArg);
+    return;
+  }
   const int rank = int(cluster_ctarank());
   const int cluster = blockIdx.x >> 1;
   const uint32_t warp = warp_id(), lane = lane_id();
 
   if (threadIdx.x == 0) {
     mbar_init(q_full, 1);
-    mbar_init(o_free, 8);
+    mbar_init(o_free, 2 * SM_WARPS);
     for (int i = 0; i < NST; ++i) {
       mbar_init(&kfull[i], 1); mbar_init(&vfull[i], 1); mbar_init(&sfull[i], 1);
-      mbar_init(&p0full[i], 8); mbar_init(&p1full[i], 4); mbar_init(&pv0[i], 1); mbar_init(&pv1[i], 1);
+      mbar_init(&p0full[i], 2 * SM_WARPS); mbar_init(&p1full[i], SM_WARPS); mbar_init(&pv0[i], 1); mbar_init(&pv1[i], 1);
     }
     *abort_flag = 0;
     fence_barrier_init();
@@ -196,7 +208,7 @@ __global__ void __launch_bounds__(256, 1) tree_mla_kernel(const __grid_constant_
   const int i0 = p.work.first[cluster], i1 = p.work.first[cluster + 1];
   auto fail = [&](int code) { if (p.status) atomicCAS(p.status, 0, code); *abort_flag = 1; };
   auto wait = [&](uint64_t* bar, uint32_t phase, int code) -> bool {
-    if (mbar_wait_cluster(bar, phase)) return true;
+    if (mbar_wait(bar, phase)) return true;
     fail(code);
     return false;
   };
@@ -204,7 +216,8 @@ __global__ void __launch_bounds__(256, 1) tree_mla_kernel(const __grid_constant_
   if (warp == 0) {
     // ---------------- producer ----------------
     if (lane == 0) {
-      tma_prefetch_desc(&tm_q); tma_prefetch_desc(&tm_kv); tma_prefetch_desc(&tm_st);
+      tma_prefetch_desc(&tm.q); tma_prefetch_desc(&tm.kv4); tma_prefetch_desc(&tm.kv1);
+      tma_prefetch_desc(&tm.st4); tma_prefetch_desc(&tm.st1);
       const uint32_t lead_q = mapa_shared(smem_u32(q_full), 0);
       int g = 0;                                        // tiles so far: stage g % 2, phase (g / 2) & 1
       bool ok = true;
@@ -213,44 +226,62 @@ __global__ void __launch_bounds__(256, 1) tree_mla_kernel(const __grid_constant_
         const int ctx = p.lay.ctx[it.b];
         const int staged_from = p.stage_all ? 0 : ctx / KT;
         const int* table = p.lay.table + size_t(it.b) * p.lay.P;
-        // 64 keys from position `pos` (a multiple of 64), dims of atom a -> a chunk
-        auto load = [&](uint8_t* dst, uint32_t bar, int tile, int half, int a) {
+        // n atoms from atom a of 64 keys (half `half` of a tile) -> chunks.  The first rows of a tile's boxes are looked
+        // up ahead of the waits: a page-table read per load would cost more than the load's issue.
+        auto row_of = [&](int tile, int half, int r) -> int {
+          if (tile >= staged_from) return (p.work.stage_at[it.b] + tile - staged_from) * KT + half * 64 + r;
+          const int pos = tile * KT + half * 64 + r;
+          return table[pos / p.lay.page] * p.lay.page + pos % p.lay.page;
+        };
+        auto load = [&](uint8_t* dst, uint32_t bar, int tile, int half, int row0, int a, bool four) {
           if (tile >= staged_from) {
-            tma_load_2d_pair(dst, &tm_st, bar, a * 64,
-                             (p.work.stage_at[it.b] + tile - staged_from) * KT + half * 64);
-          } else {
+            tma_load_3d_pair(dst, four ? &tm.st4 : &tm.st1, bar, 0, row0, a);
+          } else if (p.box == 64) {
+            tma_load_3d_pair(dst, four ? &tm.kv4 : &tm.kv1, bar, 0, row0, a);
+          } else {              // a box shorter than a chunk: one atom at a time
             for (int r = 0; r < 64; r += p.box) {
-              const int pos = tile * KT + half * 64 + r;
-              tma_load_2d_pair(dst + r * 128, &tm_kv, bar, a * 64,
-                               table[pos / p.lay.page] * p.lay.page + pos % p.lay.page);
+              const int row = r ? row_of(tile, half, r) : row0;
+              for (int k = 0; k < (four ? 4 : 1); ++k)
+                tma_load_3d_pair(dst + k * CH + r * 128, &tm.kv1, bar, 0, row, a + k);
             }
           }
+        };
+        // L2 prefetch of the CTA's half of a tile two tiles before its load: the ring holds two tiles, too few to cover
+        // the latency of HBM
+        auto prefetch = [&](int tile) {
+          if (tile >= staged_from || p.box != 64) return;
+          const int row = row_of(tile, rank, 0);
+          tma_prefetch_l2_3d(&tm.kv4, 0, row, 0);
+          tma_prefetch_l2_3d(&tm.kv4, 0, row, 4);
+          if (NA == 9) tma_prefetch_l2_3d(&tm.kv1, 0, row, 8);
         };
         // Q: the previous item's last Q·K^T is done (its V loads waited for it)
         if (rank == 0) mbar_arrive_expect_tx(q_full, 2 * NA * CH);
         const int q_row = p.lay.cu[it.b] * p.H + it.row * 128 + rank * 64;
-        for (int a = 0; a < NA; ++a) tma_load_2d_pair(sQ + a * CH, &tm_q, lead_q, a * 64, q_row);
+        tma_load_3d_pair(sQ, &tm.q, lead_q, 0, q_row, 0);
         for (int j = 0; ok && j < it.n_tiles; j += 2) {
           const int m = min(2, it.n_tiles - j);
           for (int u = 0; ok && u < m; ++u) {
             const int s = (g + u) & 1, ph = ((g + u) >> 1) & 1;
             uint8_t* st = sK + s * STAGE;
             const uint32_t bar = mapa_shared(smem_u32(&kfull[s]), 0);
+            const int tile = it.tile + j + u, row0 = row_of(tile, rank, 0);
             if (rank == 0) mbar_arrive_expect_tx(&kfull[s], 2 * NA * CH);
             if (!(ok = wait(&pv0[s], ph ^ 1, kErrTimeoutEmpty))) break;
-            for (int a = 0; a < 4; ++a) load(st + a * CH, bar, it.tile + j + u, rank, a);
-            if (NA == 9) load(st + 8 * CH, bar, it.tile + j + u, rank, 8);
+            load(st, bar, tile, rank, row0, 0, true);
+            if (NA == 9) load(st + 8 * CH, bar, tile, rank, row0, 8, false);
             if (!(ok = wait(&pv1[s], ph ^ 1, kErrTimeoutEmpty))) break;
-            for (int a = 4; a < 8; ++a) load(st + a * CH, bar, it.tile + j + u, rank, a);
+            load(st + 4 * CH, bar, tile, rank, row0, 4, true);
+            if (j + u + 2 < it.n_tiles) prefetch(tile + 2);
           }
           for (int u = 0; ok && u < m; ++u) {
             const int s = (g + u) & 1, ph = ((g + u) >> 1) & 1;
             uint8_t* st = sK + s * STAGE;
             const uint32_t bar = mapa_shared(smem_u32(&vfull[s]), 0);
+            const int tile = it.tile + j + u, row0 = row_of(tile, rank ^ 1, 0);
             if (rank == 0) mbar_arrive_expect_tx(&vfull[s], 2 * 4 * CH);
             if (!(ok = wait(&sfull[s], ph, kErrTimeoutFull))) break;
-            for (int a = 0; a < 4; ++a)
-              load(st + (rank ? a : 4 + a) * CH, bar, it.tile + j + u, rank ^ 1, 4 * rank + a);
+            load(st + (rank ? 0 : 4) * CH, bar, tile, rank ^ 1, row0, 4 * rank, true);
           }
           g += m;
         }
@@ -311,12 +342,14 @@ __global__ void __launch_bounds__(256, 1) tree_mla_kernel(const __grid_constant_
       }
     }
   } else if (warp >= 4) {
-    // ---------------- softmax, rescale, epilogue: thread = row (lanes 0-63 / 64-127: first / second 64 keys) -------
-    const int q = warp & 3, half = q >> 1, row = (q & 1) * 32 + int(lane), me = q * 32 + int(lane);
+    // ---------------- softmax, rescale, epilogue: lanes 0-63 / 64-127 hold the first / second 64 keys of the rows;
+    // two warps share 32 lanes and take 32 score columns (and 128 of the 256 columns of O) each -------
+    const int q = warp & 3, half = q >> 1, row = (q & 1) * 32 + int(lane), part = (int(warp) - 4) >> 2;
+    const int me = part * 128 + q * 32 + int(lane);
     const uint32_t t_lane = tmem + (uint32_t(q * 32) << 16);
     int g = 0;
     bool ok = true;                       // after a failed wait the loop runs on without waiting: the block-level
-    for (int i = i0; i < i1; ++i) {       // barriers below need all four warps
+    for (int i = i0; i < i1; ++i) {       // barriers below need all the warps
       const TreeItem it = p.work.items[i];
       const int ctx = p.lay.ctx[it.b], c0 = p.lay.cu[it.b], n = p.lay.cu[it.b + 1] - c0;
       const int r = it.row * 128 + rank * 64 + row;
@@ -328,29 +361,28 @@ __global__ void __launch_bounds__(256, 1) tree_mla_kernel(const __grid_constant_
         const int s = g & 1, ph = (g >> 1) & 1;
         ok = ok && wait(&sfull[s], ph, kErrTimeoutTmem);
         tc_fence_after();
-        uint32_t x[64];
-        tmem_ld_32x32b_x32(t_lane + TM_S + s * 64, *reinterpret_cast<uint32_t(*)[32]>(&x[0]));
-        tmem_ld_32x32b_x32(t_lane + TM_S + s * 64 + 32, *reinterpret_cast<uint32_t(*)[32]>(&x[32]));
+        uint32_t x[32];
+        tmem_ld_32x32b_x32(t_lane + TM_S + s * 64 + part * 32, x);
         tmem_ld_wait();
-        const int first = (it.tile + j) * KT + half * 64;       // position of this thread's first key
-        if (first + 64 > ctx) {
-          const int off = ctx - first;                          // keys before the tree
-          const uint64_t pre = off <= 0 ? 0 : (uint64_t(1) << off) - 1;
-          const uint64_t see = pre | (off >= 0 ? mask << off : (off > -64 ? mask >> -off : 0));
+        const int first = (it.tile + j) * KT + half * 64 + part * 32;   // position of this thread's first key
+        if (first + 32 > ctx) {
+          const int off = ctx - first;                                  // keys before the tree
+          const uint32_t pre = off <= 0 ? 0 : (1u << off) - 1;
+          const uint32_t see = pre | uint32_t(off >= 0 ? mask << off : (off > -64 ? mask >> -off : 0));
 #pragma unroll
-          for (int k = 0; k < 64; ++k)
+          for (int k = 0; k < 32; ++k)
             if (!((see >> k) & 1)) x[k] = 0xff800000u;
         }
         float m0 = -INFINITY, m1 = -INFINITY, m2 = -INFINITY, m3 = -INFINITY;
 #pragma unroll
-        for (int k = 0; k < 64; k += 4) {
+        for (int k = 0; k < 32; k += 4) {
           m0 = fmaxf(m0, __uint_as_float(x[k])); m1 = fmaxf(m1, __uint_as_float(x[k + 1]));
           m2 = fmaxf(m2, __uint_as_float(x[k + 2])); m3 = fmaxf(m3, __uint_as_float(x[k + 3]));
         }
-        float mt = fmaxf(fmaxf(m0, m1), fmaxf(m2, m3));
-        xm[(g & 1) * 128 + me] = mt;
+        float* xb = xm + (g & 1) * 256;
+        xb[me] = fmaxf(fmaxf(m0, m1), fmaxf(m2, m3));
         softmax_sync();
-        mt = fmaxf(mt, xm[(g & 1) * 128 + (me ^ 64)]) * p.scale_log2;
+        const float mt = fmaxf(fmaxf(xb[me], xb[me ^ 64]), fmaxf(xb[me ^ 128], xb[me ^ 192])) * p.scale_log2;
         const bool grow = j > 0 && mt > m_used + kRescale;
         const float m_new = grow || j == 0 ? fmaxf(m_used, mt) : m_used;
         const float m_ref = m_new == -INFINITY ? 0.f : m_new;
@@ -359,7 +391,7 @@ __global__ void __launch_bounds__(256, 1) tree_mla_kernel(const __grid_constant_
           ok = ok && wait(&pv1[s ^ 1], ((g - 1) >> 1) & 1, kErrTimeoutTmem);
           tc_fence_after();
 #pragma unroll 1
-          for (int c = 0; c < 256; c += 32) {
+          for (int c = part * 128; c < part * 128 + 128; c += 32) {
             uint32_t o[32];
             tmem_ld_32x32b_x32(t_lane + TM_O + c, o);
             tmem_ld_wait();
@@ -373,7 +405,7 @@ __global__ void __launch_bounds__(256, 1) tree_mla_kernel(const __grid_constant_
         m_used = m_new;
         float l0 = 0.f, l1 = 0.f;
 #pragma unroll
-        for (int k = 0; k < 64; k += 2) {
+        for (int k = 0; k < 32; k += 2) {
           const float a = ex2(fmaf(__uint_as_float(x[k]), p.scale_log2, -m_ref));
           const float b = ex2(fmaf(__uint_as_float(x[k + 1]), p.scale_log2, -m_ref));
           l0 += a;
@@ -384,18 +416,18 @@ __global__ void __launch_bounds__(256, 1) tree_mla_kernel(const __grid_constant_
         tc_fence_before();
         if (half) {
           __syncwarp();
-          if (lane == 0) mbar_arrive_cluster_release(mapa_shared(smem_u32(&p0full[s]), 0));   // scores read, O rescaled
+          if (lane == 0) mbar_arrive_cluster(mapa_shared(smem_u32(&p0full[s]), 0));   // scores read, O rescaled
           // the extra chunk: the previous tile's P·V must have read it
           ok = ok && wait(&pv1[s ^ 1], ((g - 1) >> 1) & 1, kErrTimeoutTmem);
         }
         uint8_t* dst = (half ? sX : sK + s * STAGE + 8 * CH) + row * 128;
 #pragma unroll
-        for (int c = 0; c < 8; ++c)
-          *reinterpret_cast<uint4*>(dst + ((c ^ (row & 7)) << 4)) =
+        for (int c = 0; c < 4; ++c)
+          *reinterpret_cast<uint4*>(dst + (((part * 4 + c) ^ (row & 7)) << 4)) =
               make_uint4(x[4 * c], x[4 * c + 1], x[4 * c + 2], x[4 * c + 3]);
         fence_proxy_async();
         __syncwarp();
-        if (lane == 0) mbar_arrive_cluster_release(mapa_shared(smem_u32(half ? &p1full[s] : &p0full[s]), 0));
+        if (lane == 0) mbar_arrive_cluster(mapa_shared(smem_u32(half ? &p1full[s] : &p0full[s]), 0));
       }
       // ---- item's end
       const int sl = (g - 1) & 1;
@@ -406,24 +438,28 @@ __global__ void __launch_bounds__(256, 1) tree_mla_kernel(const __grid_constant_
         const uint64_t bad = uint64_t(__ballot_sync(~0u, b0)) | uint64_t(__ballot_sync(~0u, b1)) << 32;
         if (mask & bad) l = __int_as_float(0x7fffffff);
       }
-      xm[256 + me] = l;
+      // sums: the maxima buffer of the tile before last is free, and the next item's first tile takes it only after
+      // every warp passed the second barrier
+      float* xs = xm + (g & 1) * 256;
+      xs[me] = l;
       softmax_sync();
-      l += xm[256 + (me ^ 64)];
+      l = (xs[me] + xs[me ^ 64]) + (xs[me ^ 128] + xs[me ^ 192]);
+      softmax_sync();
       float inv = 1.f;
       if (it.part < 0) {
         if (p.sink && live) l += exp2f(p.sink[head] * 1.4426950408889634f - (m_used == -INFINITY ? 0.f : m_used));
         inv = l == 0.f ? 0.f : 1.f / l;
-      } else if (half == 0) {
+      } else if (half == 0 && part == 0) {
         float* ml = p.part_ml + (size_t(it.part) * 128 + rank * 64 + row) * 2;
         ml[0] = m_used;
         ml[1] = l;
       }
-      __nv_bfloat16* o = p.out + (size_t(c0) * p.H + r) * 512 + half * 256;
-      float* po = p.part_o + (size_t(max(it.part, 0)) * 128 + rank * 64 + row) * 512 + half * 256;
+      __nv_bfloat16* o = p.out + (size_t(c0) * p.H + r) * 512 + half * 256 + part * 128;
+      float* po = p.part_o + (size_t(max(it.part, 0)) * 128 + rank * 64 + row) * 512 + half * 256 + part * 128;
 #pragma unroll 1
-      for (int c = 0; c < 256; c += 32) {
+      for (int c = 0; c < 128; c += 32) {
         uint32_t v[32];
-        tmem_ld_32x32b_x32(t_lane + TM_O + c, v);
+        tmem_ld_32x32b_x32(t_lane + TM_O + part * 128 + c, v);
         tmem_ld_wait();
         if (it.part >= 0) {
 #pragma unroll
@@ -441,7 +477,7 @@ __global__ void __launch_bounds__(256, 1) tree_mla_kernel(const __grid_constant_
       }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive_cluster_release(mapa_shared(smem_u32(o_free), 0));
+      if (lane == 0) mbar_arrive_cluster(mapa_shared(smem_u32(o_free), 0));
     }
   }
   __syncthreads();
@@ -502,18 +538,18 @@ static PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
   return fn;
 }
 
-// [rows, D] 16-bit row-major matrix read in boxes of box_rows x 64
-static bool row_map(CUtensorMap* m, bool f16, const void* base, int64_t rows, int D, int box_rows) {
-  const cuuint64_t dims[2] = {cuuint64_t(D), cuuint64_t(rows)};
-  const cuuint64_t str[1] = {cuuint64_t(D) * 2};
-  const cuuint32_t box[2] = {64, cuuint32_t(box_rows)}, es[2] = {1, 1};
-  return encode_fn()(m, f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2,
+// [rows, D] 16-bit row-major matrix as (64, rows, D / 64), read in boxes of 64 x box_rows x atoms
+static bool row_map(CUtensorMap* m, bool f16, const void* base, int64_t rows, int D, int box_rows, int atoms) {
+  const cuuint64_t dims[3] = {64, cuuint64_t(rows), cuuint64_t(D) / 64};
+  const cuuint64_t str[2] = {cuuint64_t(D) * 2, 128};
+  const cuuint32_t box[3] = {64, cuuint32_t(box_rows), cuuint32_t(atoms)}, es[3] = {1, 1, 1};
+  return encode_fn()(m, f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3,
                      const_cast<void*>(base), dims, str, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
                      CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-using Kernel = void (*)(const CUtensorMap, const CUtensorMap, const CUtensorMap, const Params);
+using Kernel = void (*)(const Maps, const Params);
 
 static cudaLaunchConfig_t pair_config(int clusters, cudaLaunchAttribute* attr, cudaStream_t s) {
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -522,7 +558,7 @@ static cudaLaunchConfig_t pair_config(int clusters, cudaLaunchAttribute* attr, c
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(2 * clusters);
-  cfg.blockDim = dim3(256);
+  cfg.blockDim = dim3(THREADS);
   cfg.dynamicSmemBytes = SMEM;
   cfg.stream = s;
   cfg.attrs = attr;
@@ -551,11 +587,15 @@ cudaError_t tree_mla(const void* q, int T, int H, int D, bool f8, bool all, cons
   int box = 64;
   while (lay.page % box) box /= 2;
   if (box < 8 && !all) return cudaErrorInvalidValue;
-  CUtensorMap tq, tkv, tst;
-  if (!row_map(&tq, f8, q, int64_t(T) * H, D, 64) || !row_map(&tst, f8, staged, int64_t(work.n_stage) * KT, D, 64))
+  Maps m;
+  const int64_t st_rows = int64_t(work.n_stage) * KT;
+  if (!row_map(&m.q, f8, q, int64_t(T) * H, D, 64, D / 64) || !row_map(&m.st4, f8, staged, st_rows, D, 64, 4) ||
+      !row_map(&m.st1, f8, staged, st_rows, D, 64, 1))
     return cudaErrorInvalidValue;
-  if (all) tkv = tst;
-  else if (!row_map(&tkv, false, kv, S, D, box)) return cudaErrorInvalidValue;
+  m.kv4 = m.st4;
+  m.kv1 = m.st1;
+  if (!all && !(row_map(&m.kv4, false, kv, S, D, box, 4) && row_map(&m.kv1, false, kv, S, D, box, 1)))
+    return cudaErrorInvalidValue;
   const auto* kvb = reinterpret_cast<const uint8_t*>(kv);
   auto* st = reinterpret_cast<uint16_t*>(staged);
   cudaError_t e = launch_k(f8 ? tree_stage_kernel<true> : tree_stage_kernel<false>, dim3(work.n_stage * 4), 256, 0, s,
@@ -572,7 +612,7 @@ cudaError_t tree_mla(const void* q, int T, int H, int D, bool f8, bool all, cons
   if ((e = smem_optin(f, SMEM)) != cudaSuccess) return e;
   cudaLaunchAttribute attr[2];
   const cudaLaunchConfig_t cfg = pair_config(work.clusters, attr, s);
-  if ((e = cudaLaunchKernelEx(&cfg, f, tq, tkv, tst, p)) != cudaSuccess || !work.n_merges) return e;
+  if ((e = cudaLaunchKernelEx(&cfg, f, m, p)) != cudaSuccess || !work.n_merges) return e;
   return launch_k(tree_merge_kernel, dim3(work.n_merges, 16), 256, 0, s, lay, work.merges, H, part_o, part_ml, sink,
                   p.out);
 }
