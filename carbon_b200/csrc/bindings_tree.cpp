@@ -28,15 +28,16 @@ cb::TreeLayout layout(const Tensor& cu, const Tensor& ctx, const Tensor& table, 
 }
 
 // Split of one attention call over `clusters` CTA pairs (csrc/tree.h: TreeWork).  Every row tile of every request is a
-// list of ceil((ctx + n) / 128) key tiles; longest first, each goes to the pair with the least work so far, and where it
-// would pass the even share it is cut there and the rest goes on to the next pair (partial results are merged).  The
-// row tiles of a request are handed out one after the other, so they run at about the same time and read its keys from
-// L2.  kOver: cost of an item's start and end in key tiles.
+// list of ceil((ctx + n) / 128) key tiles; longest first, each goes to the pair with the least work so far.  Where it
+// would pass the even share it is cut there and the rest goes on to the next pair (partial results are merged); the
+// share grows a little until no piece comes out shorter than kPiece.  The row tiles of a request are handed out one
+// after the other, so they run at about the same time and read its keys from L2.  kOver: cost of an item's start and
+// end in key tiles.
 // -> int32 tensor: first [clusters + 1], items [*, 5], merges [*, 4], (even offset) staged blocks of the tail mode
 // [*, 2], of the all mode [*, 2], first block per request of either [B] [B]; and the counts
 std::tuple<Tensor, std::vector<int64_t>> tree_schedule(const std::vector<int64_t>& n, const std::vector<int64_t>& ctx,
                                                        int64_t H, int64_t clusters) {
-  constexpr int64_t kTile = 128, kOver = 2;
+  constexpr int64_t kTile = 128, kOver = 2, kPiece = 2;
   const int64_t B = int64_t(n.size());
   struct Row { int64_t b, row, tiles; };
   std::vector<Row> rows;
@@ -47,33 +48,42 @@ std::tuple<Tensor, std::vector<int64_t>> tree_schedule(const std::vector<int64_t
   }
   std::stable_sort(rows.begin(), rows.end(), [](const Row& x, const Row& y) { return x.tiles > y.tiles; });
   clusters = std::max<int64_t>(1, clusters);
-  const int64_t share = (total + clusters - 1) / clusters;
   using Load = std::pair<int64_t, int64_t>;                       // (work, pair)
-  std::priority_queue<Load, std::vector<Load>, std::greater<Load>> heap;
-  for (int64_t c = 0; c < clusters; ++c) heap.push({0, c});
-  std::vector<std::vector<cb::TreeItem>> lists(clusters);
+  std::vector<std::vector<cb::TreeItem>> lists;
   std::vector<cb::TreeMerge> merges;
   int64_t parts = 0;
-  for (const Row& r : rows) {
-    int64_t at = 0;
-    const int64_t first_part = parts;
-    std::vector<std::pair<int64_t, size_t>> pieces;
-    while (at < r.tiles) {
-      const Load ld = heap.top();
-      heap.pop();
-      const int64_t rest = r.tiles - at, room = std::max<int64_t>(1, share - ld.first - kOver);
-      const int64_t take = rest <= room + 1 ? rest : room;
-      auto& list = lists[ld.second];
-      pieces.push_back({ld.second, list.size()});
-      list.push_back({int(r.b), int(r.row), int(at), int(take), -1});
-      heap.push({ld.first + take + kOver, ld.second});
-      at += take;
+  auto assign = [&](int64_t share, bool force) -> bool {
+    std::priority_queue<Load, std::vector<Load>, std::greater<Load>> heap;
+    for (int64_t c = 0; c < clusters; ++c) heap.push({0, c});
+    lists.assign(clusters, {});
+    merges.clear();
+    parts = 0;
+    for (const Row& r : rows) {
+      const int64_t first_part = parts;
+      std::vector<std::pair<int64_t, size_t>> pieces;
+      for (int64_t at = 0; at < r.tiles;) {
+        const Load ld = heap.top();
+        heap.pop();
+        const int64_t rest = r.tiles - at, room = share - ld.first - kOver;
+        if (!force && room < std::min(rest, kPiece)) return false;
+        // a remainder shorter than a piece stays here
+        const int64_t take = force || rest < room + std::min(kPiece, share / 16 + 1) ? rest : room;
+        auto& list = lists[ld.second];
+        pieces.push_back({ld.second, list.size()});
+        list.push_back({int(r.b), int(r.row), int(at), int(take), -1});
+        heap.push({ld.first + take + kOver, ld.second});
+        at += take;
+      }
+      if (pieces.size() > 1) {
+        for (auto& [c, i] : pieces) lists[c][i].part = int(parts++);
+        merges.push_back({int(r.b), int(r.row), int(first_part), int(pieces.size())});
+      }
     }
-    if (pieces.size() > 1) {
-      for (auto& [c, i] : pieces) lists[c][i].part = int(parts++);
-      merges.push_back({int(r.b), int(r.row), int(first_part), int(pieces.size())});
-    }
-  }
+    return true;
+  };
+  int64_t share = std::max((total + clusters - 1) / clusters, kPiece + kOver);
+  int tries = 0;
+  while (!assign(share, ++tries > 60)) share += std::max<int64_t>(1, share / 40);
   int64_t used = 0, n_items = 0, n_tail = 0, n_all = 0;
   for (auto& l : lists) { used += !l.empty(); n_items += int64_t(l.size()); }
   std::stable_sort(lists.begin(), lists.end(), [](const auto& x, const auto& y) { return !x.empty() && y.empty(); });

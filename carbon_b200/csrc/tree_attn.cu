@@ -320,20 +320,21 @@ __global__ void __launch_bounds__(THREADS, 1) tree_mla_kernel(const __grid_const
             if (!ok) break;
             tc_fence_after();
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-#pragma unroll
-              for (int c = 0; c < 2; ++c)
-                mma_f16_ss_pair(tmem + TM_O + c * 128, smem_desc_sw128(st + 8 * CH + k * 32),
-                                desc_mn(st + 2 * c * CH + k * 2048), id_pv, (j + u > 0 || k > 0) ? 1u : 0u);
+            for (int k = 0; k < 4; ++k) {
+              const uint64_t a = smem_desc_sw128(st + 8 * CH + k * 32);
+              const uint32_t acc = (j + u > 0 || k > 0) ? 1u : 0u;
+              mma_f16_ss_pair_keep_a(tmem + TM_O, a, desc_mn(st + k * 2048), id_pv, acc);
+              mma_f16_ss_pair_last_a(tmem + TM_O + 128, a, desc_mn(st + 2 * CH + k * 2048), id_pv, acc);
+            }
             mma_commit_pair(&pv0[s], 3);
             if (!(ok = wait(&p1full[s], ph, kErrTimeoutTmem))) break;
             tc_fence_after();
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-#pragma unroll
-              for (int c = 0; c < 2; ++c)
-                mma_f16_ss_pair(tmem + TM_O + c * 128, smem_desc_sw128(sX + k * 32),
-                                desc_mn(st + (4 + 2 * c) * CH + k * 2048), id_pv, 1u);
+            for (int k = 0; k < 4; ++k) {
+              const uint64_t a = smem_desc_sw128(sX + k * 32);
+              mma_f16_ss_pair_keep_a(tmem + TM_O, a, desc_mn(st + 4 * CH + k * 2048), id_pv, 1u);
+              mma_f16_ss_pair_last_a(tmem + TM_O + 128, a, desc_mn(st + 6 * CH + k * 2048), id_pv, 1u);
+            }
             mma_commit_pair(&pv1[s], 3);
           }
           g += m;
@@ -488,43 +489,38 @@ __global__ void __launch_bounds__(THREADS, 1) tree_mla_kernel(const __grid_const
 #endif
 }
 
-// out = sum_s 2^(m_s - M) O_s / (sum_s 2^(m_s - M) l_s + sink): one warp per row of a split row tile.
-__global__ void __launch_bounds__(256) tree_merge_kernel(TreeLayout lay, const TreeMerge* __restrict__ merges, int H,
+// out = sum_s 2^(m_s - M) O_s / (sum_s 2^(m_s - M) l_s + sink): one CTA per row of a split row tile, four of the 512
+// dims per thread, eight partial rows in flight.
+__global__ void __launch_bounds__(128) tree_merge_kernel(TreeLayout lay, const TreeMerge* __restrict__ merges, int H,
                                                          const float* __restrict__ part_o,
                                                          const float* __restrict__ part_ml,
                                                          const float* __restrict__ sink,
                                                          __nv_bfloat16* __restrict__ out) {
   pdl_entry();
   const TreeMerge mg = merges[blockIdx.x];
-  const int row = blockIdx.y * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  const int row = blockIdx.y;
   const int r = mg.row * 128 + row, n = lay.cu[mg.b + 1] - lay.cu[mg.b];
   if (r >= n * H) return;
-  const int head = r % H;
   const float2* ml = reinterpret_cast<const float2*>(part_ml) + size_t(mg.part) * 128 + row;
-  float M = sink ? sink[head] * 1.4426950408889634f : -INFINITY;
+  const float sk = sink ? sink[r % H] * 1.4426950408889634f : -INFINITY;
+  float M = sk;
+#pragma unroll 8
   for (int s = 0; s < mg.n; ++s) M = fmaxf(M, ml[s * 128].x);
   if (M == -INFINITY) M = 0.f;
-  float L = sink ? exp2f(sink[head] * 1.4426950408889634f - M) : 0.f;
-  float acc[16];
-#pragma unroll
-  for (int k = 0; k < 16; ++k) acc[k] = 0.f;
-  const float* po = part_o + (size_t(mg.part) * 128 + row) * 512 + lane * 4;
+  float L = exp2f(sk - M);
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  const float4* po = reinterpret_cast<const float4*>(part_o) + (size_t(mg.part) * 128 + row) * 128 + threadIdx.x;
+#pragma unroll 8
   for (int s = 0; s < mg.n; ++s) {
     const float2 v = ml[s * 128];
+    const float4 o = po[size_t(s) * 128 * 128];
     const float w = exp2f(v.x - M);
     L += w * v.y;
-#pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      const float4 o = *reinterpret_cast<const float4*>(po + size_t(s) * 128 * 512 + c * 128);
-      acc[4 * c] += w * o.x; acc[4 * c + 1] += w * o.y; acc[4 * c + 2] += w * o.z; acc[4 * c + 3] += w * o.w;
-    }
+    acc.x += w * o.x; acc.y += w * o.y; acc.z += w * o.z; acc.w += w * o.w;
   }
   const float inv = L == 0.f ? 0.f : 1.f / L;
-  __nv_bfloat16* o = out + (size_t(lay.cu[mg.b]) * H + r) * 512 + lane * 4;
-#pragma unroll
-  for (int c = 0; c < 4; ++c)
-    *reinterpret_cast<uint2*>(o + c * 128) = make_uint2(pack_bf16x2(acc[4 * c] * inv, acc[4 * c + 1] * inv),
-                                                        pack_bf16x2(acc[4 * c + 2] * inv, acc[4 * c + 3] * inv));
+  reinterpret_cast<uint2*>(out + (size_t(lay.cu[mg.b]) * H + r) * 512)[threadIdx.x] =
+      make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
 }
 
 static PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
@@ -613,7 +609,7 @@ cudaError_t tree_mla(const void* q, int T, int H, int D, bool f8, bool all, cons
   cudaLaunchAttribute attr[2];
   const cudaLaunchConfig_t cfg = pair_config(work.clusters, attr, s);
   if ((e = cudaLaunchKernelEx(&cfg, f, m, p)) != cudaSuccess || !work.n_merges) return e;
-  return launch_k(tree_merge_kernel, dim3(work.n_merges, 16), 256, 0, s, lay, work.merges, H, part_o, part_ml, sink,
+  return launch_k(tree_merge_kernel, dim3(work.n_merges, 128), 128, 0, s, lay, work.merges, H, part_o, part_ml, sink,
                   p.out);
 }
 
