@@ -4,137 +4,267 @@
 // remainder r starts as p; child c (index order) is accepted when u_c q(x_c) < r(x_c), q the distribution its token was
 // drawn from; a rejection leaves r <- max(r - q, 0) / (its sum).  Where no child is accepted the next token is
 // argmax_i r_i / e_i with e ~ Exp(1) given, which is a draw from r.  Sums, maxima and probabilities are fp32.
-#include "common.cuh"
+#include "ptx.cuh"
 #include "tree.h"
 
 namespace cb {
 namespace tree {
 
-constexpr int kNodes = 64;
+constexpr int kNodes = 64, kThreads = 512, kUnroll = 8, kMaxCluster = 16;
+constexpr float kLog2e = 1.4426950408889634f;
 
-template <bool BF16>
-CB_DEVICE float logit(const void* l, int64_t i) {
-  if constexpr (BF16) return __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(l)[i]);
-  else return reinterpret_cast<const float*>(l)[i];
+CB_DEVICE float ex2v(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
 
-// (value, index) maximum over the block, ties to the lowest index; index -1 = none
-CB_DEVICE void block_argmax(float& v, int& i, float* sv, int* si) {
-  const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5, nw = blockDim.x >> 5;
-  auto take = [&](float ov, int oi) {
-    if (oi >= 0 && (i < 0 || ov > v || (ov == v && oi < i))) { v = ov; i = oi; }
-  };
-  for (int o = 16; o; o >>= 1) take(__shfl_xor_sync(~0u, v, o), __shfl_xor_sync(~0u, i, o));
-  __syncthreads();
-  if (lane == 0) { sv[wid] = v; si[wid] = i; }
-  __syncthreads();
-  v = lane < nw ? sv[lane] : 0.f;
-  i = lane < nw ? si[lane] : -1;
-  for (int o = 16; o; o >>= 1) take(__shfl_xor_sync(~0u, v, o), __shfl_xor_sync(~0u, i, o));
-}
+// One row slice's statistics: maximum, its lowest index, sum of 2^((l - max) k).
+struct Stat {
+  float m, s;
+  int i;
+  CB_DEVICE void join(const Stat& o, float k) {
+    if (o.i < 0) return;
+    if (i < 0) { *this = o; return; }
+    const float t = fmaxf(m, o.m), ref = t == -INFINITY ? 0.f : t;
+    s = s * ex2v((m - ref) * k) + o.s * ex2v((o.m - ref) * k);
+    if (o.m > m || (o.m == m && o.i < i)) i = o.i;
+    m = t;
+  }
+};
 
-template <bool BF16>
-__global__ void __launch_bounds__(1024) tree_verify_kernel(const void* __restrict__ logits, int64_t ld, int V,
-                                                           const int* __restrict__ tokens, const int* __restrict__ cu,
-                                                           const int* __restrict__ parent, int N,
-                                                           const float* __restrict__ uniforms,
-                                                           const float* __restrict__ noise,
-                                                           const float* __restrict__ temperature,
-                                                           const float* __restrict__ draft, int* __restrict__ path,
-                                                           int* __restrict__ n_accepted, int* __restrict__ out_tokens,
-                                                           float* __restrict__ logprobs) {
+// Reductions over the threads of all CTAs of the cluster; every thread gets the result.  A CTA's value goes to every
+// CTA's slot array through distributed shared memory; two arrays alternate, so that one exchange's slots are read
+// before the next but one writes them.
+struct Exchange {
+  float4 (*slots)[kMaxCluster];     // [2][kMaxCluster]
+  float4* warps;                    // [kThreads / 32]
+  int n, rank, turn;
+  // value of the block (in all threads of warp 0) -> all CTAs
+  CB_DEVICE void all(float4 v) {
+    const int t = turn & 1;
+    if (n == 1) {
+      if (threadIdx.x == 0) slots[t][0] = v;
+      __syncthreads();
+    } else {
+      if (threadIdx.x < uint32_t(n))
+        st_cluster_v4(mapa_shared(smem_u32(&slots[t][rank]), threadIdx.x), __float_as_uint(v.x), __float_as_uint(v.y),
+                      __float_as_uint(v.z), __float_as_uint(v.w));
+      cluster_sync();
+    }
+  }
+  template <typename F>
+  CB_DEVICE float4 reduce(float4 v, F join) {
+    const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
+#pragma unroll
+    for (int o = 16; o; o >>= 1)
+      join(v, make_float4(__shfl_xor_sync(~0u, v.x, o), __shfl_xor_sync(~0u, v.y, o), __shfl_xor_sync(~0u, v.z, o),
+                          __shfl_xor_sync(~0u, v.w, o)));
+    if (lane == 0) warps[wid] = v;
+    __syncthreads();
+    if (wid == 0) {
+      v = warps[lane & (kThreads / 32 - 1)];
+#pragma unroll
+      for (int o = kThreads / 64; o; o >>= 1)
+        join(v, make_float4(__shfl_xor_sync(~0u, v.x, o), __shfl_xor_sync(~0u, v.y, o), __shfl_xor_sync(~0u, v.z, o),
+                            __shfl_xor_sync(~0u, v.w, o)));
+    }
+    all(v);
+    const int t = turn++ & 1;
+    v = slots[t][0];
+    for (int c = 1; c < n; ++c) join(v, slots[t][c]);
+    return v;
+  }
+  CB_DEVICE Stat stat(const Stat& a, float k) {
+    const float4 r = reduce(make_float4(a.m, a.s, __int_as_float(a.i), 0.f), [&](float4& x, const float4& y) {
+      Stat p{x.x, x.y, __float_as_int(x.z)};
+      p.join(Stat{y.x, y.y, __float_as_int(y.z)}, k);
+      x = make_float4(p.m, p.s, __int_as_float(p.i), 0.f);
+    });
+    return Stat{r.x, r.y, __float_as_int(r.z)};
+  }
+  // maxima of two scores at once, lowest index among equals (index -1: none)
+  CB_DEVICE float4 best2(float4 a) {
+    return reduce(a, [](float4& x, const float4& y) {
+      auto take = [](float& v, float& i, float ov, float oi) {
+        const int a = __float_as_int(i), b = __float_as_int(oi);
+        if (b >= 0 && (a < 0 || ov > v || (ov == v && b < a))) { v = ov; i = oi; }
+      };
+      take(x.x, x.y, y.x, y.y);
+      take(x.z, x.w, y.z, y.w);
+    });
+  }
+  CB_DEVICE float sum(float a) {
+    return reduce(make_float4(a, 0.f, 0.f, 0.f), [](float4& x, const float4& y) { x.x += y.x; }).x;
+  }
+};
+
+// One cluster per request: its CTAs share the vocabulary.  A visited node costs one pass over its logits; a rejection
+// of a token drawn from a distribution one pass over logits and distribution for the remainder's sum (not needed for
+// the last child, whose remainder goes straight into the draw); the end one pass over logits, distribution and noise.
+template <bool BF16, bool DRAFT>
+__global__ void __launch_bounds__(kThreads) tree_verify_kernel(
+    const void* __restrict__ logits, int64_t ld, int V, const int* __restrict__ tokens, const int* __restrict__ cu,
+    const int* __restrict__ parent, int N, const float* __restrict__ uniforms, const float* __restrict__ noise,
+    const float* __restrict__ temperature, const float* __restrict__ draft, int clusters, int* __restrict__ path,
+    int* __restrict__ n_accepted, int* __restrict__ out_tokens, float* __restrict__ logprobs) {
   pdl_entry();
-  __shared__ float red[32], red2[32];
-  __shared__ int redi[32];
-  __shared__ int s_tok[kNodes], s_par[kNodes];
-  __shared__ float s_u[kNodes];
-  const int b = blockIdx.x, t0 = cu[b], n = cu[b + 1] - t0;
-  for (int i = threadIdx.x; i < N; i += blockDim.x) {
-    path[b * N + i] = -1;
-    out_tokens[b * N + i] = -1;
-    logprobs[b * N + i] = 0.f;
+  __shared__ float4 sh_slots[2][kMaxCluster], sh_warps[kThreads / 32];
+  __shared__ int s_tok[kNodes], s_par[kNodes], s_gone[kNodes];
+  __shared__ float s_u[kNodes], s_l[kNodes], s_q[kNodes], s_mass[kNodes];
+  const int n_cta = gridDim.x / clusters;
+  const int rank = n_cta == 1 ? 0 : int(cluster_ctarank()), b = blockIdx.x / n_cta;
+  Exchange ex{sh_slots, sh_warps, n_cta, rank, 0};
+  const int t0 = cu[b], n = cu[b + 1] - t0;
+  for (int i = threadIdx.x; i < N; i += kThreads) {
+    if (rank == 0) {
+      path[b * N + i] = -1;
+      out_tokens[b * N + i] = -1;
+      logprobs[b * N + i] = 0.f;
+    }
     if (i < n) { s_tok[i] = tokens[t0 + i]; s_par[i] = parent[t0 + i]; s_u[i] = uniforms[t0 + i]; }
   }
-  __syncthreads();
+  if (n_cta > 1) cluster_sync();                       // every CTA runs before any remote store
+  else __syncthreads();
   if (n <= 0) {
-    if (threadIdx.x == 0) n_accepted[b] = -1;
+    if (threadIdx.x == 0 && rank == 0) n_accepted[b] = -1;
     return;
   }
   const float T = temperature[b];
   const bool greedy = !(T > 0.f);
-  const float heat = greedy ? 1.f : T;
-  float mass[kNodes];                       // of this node's rejections, in order
-  int gone[kNodes];                         // their tokens
+  const float k = greedy ? kLog2e : kLog2e / T;        // p = 2^((l - max) k) / total
+  const int per = (V + n_cta - 1) / n_cta, lo = rank * per, hi = min(V, lo + per);
   int v = 0, steps = 0;
   while (true) {
-    const char* row = reinterpret_cast<const char*>(logits) + (size_t(t0 + v) * ld) * (BF16 ? 2 : 4);
-    const float* q = draft ? draft + size_t(t0 + v) * V : nullptr;
-    float top = -INFINITY;
-    int best = -1;
-    for (int i = threadIdx.x; i < V; i += blockDim.x) {
-      const float l = logit<BF16>(row, i);
-      if (best < 0 || l > top) { top = l; best = i; }
+    const char* rowp = reinterpret_cast<const char*>(logits) + (size_t(t0 + v) * ld) * (BF16 ? 2 : 4);
+    const float* q = DRAFT ? draft + size_t(t0 + v) * V : nullptr;
+    const float* e = noise + size_t(b) * V;
+    auto logit = [&](int i) -> float {
+      if constexpr (BF16) return __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(rowp)[i]);
+      else return reinterpret_cast<const float*>(rowp)[i];
+    };
+    // the children's logits and draft probabilities, read while the pass runs
+    int last = -1;                                     // the last child
+    for (int c = v + 1; c < n; ++c)
+      if (s_par[c] == v) last = c;
+    if (int(threadIdx.x) < n && s_par[threadIdx.x] == v) {
+      const int x = s_tok[threadIdx.x];
+      const bool in = x >= 0 && x < V;
+      s_l[threadIdx.x] = in ? logit(x) : -INFINITY;
+      s_q[threadIdx.x] = in ? (DRAFT ? q[x] : 1.f) : -1.f;      // no such token: never accepted
     }
-    block_argmax(top, best, red, redi);
-    const float smax = top / heat;
-    const float ref = smax == -INFINITY ? 0.f : smax;
-    float e = 0.f;
-    for (int i = threadIdx.x; i < V; i += blockDim.x) e += expf(logit<BF16>(row, i) / heat - ref);
-    const float total = block_sum(e, red2);
-    const float denom = total > 0.f ? total : (total == total ? 1.f : total);
-    int k = 0;
-    // remainder of token i after this node's k rejections
-    auto rest = [&](int i) -> float {
-      if (greedy) return i == best && total > 0.f ? 1.f : 0.f;
-      float r = expf(logit<BF16>(row, i) / heat - ref) / denom;
-      for (int j = 0; j < k; ++j) {
-        if (q) r = fmaxf(r - q[i], 0.f) / mass[j];
-        else r = gone[j] == i ? 0.f : r / mass[j];
-      }
+    Stat st{-INFINITY, 0.f, -1};
+    for (int i0 = lo + int(threadIdx.x); i0 < hi; i0 += kThreads * kUnroll) {
+      float x[kUnroll];
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) x[u] = i0 + u * kThreads < hi ? logit(i0 + u * kThreads) : -INFINITY;
+      float m = st.m;
+      int at = st.i < 0 ? i0 : st.i;
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u)
+        if (x[u] > m) { m = x[u]; at = i0 + u * kThreads; }
+      const float ref = m == -INFINITY ? 0.f : m;
+      float s = st.s * ex2v((st.m - ref) * k);
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) s += ex2v((x[u] - ref) * k);
+      st = Stat{m, s, at};
+    }
+    st = ex.stat(st, k);
+    const float ref = st.m == -INFINITY ? 0.f : st.m, total = st.s;
+    const float inv = total > 0.f ? 1.f / total : (total == total ? 0.f : total);
+    const int best = total > 0.f ? st.i : -1;
+    const float lse = log2f(total);
+    auto logprob = [&](float l) { return ((l - ref) * k - lse) * 0.6931471805599453f; };
+    int gone = 0;                                      // rejections that changed the remainder
+    // remainder of token i with logit l after them
+    auto rest = [&](int i, float l, float qi) -> float {
+      if (greedy) return i == best ? 1.f : 0.f;
+      float r = ex2v((l - ref) * k) * inv;
+      for (int j = 0; j < gone; ++j) r = DRAFT ? fmaxf(r - qi, 0.f) * s_mass[j] : (s_gone[j] == i ? 0.f : r * s_mass[j]);
       return r;
     };
     int next = -1, x = -1;
-    for (int c = v + 1; c < n && next < 0; ++c) {
+    bool open = false;                                 // the last child's rejection goes into the draw
+    float left = 1.f;                                  // mass of the certain proposals' remainder
+    for (int c = v + 1; c <= last && next < 0; ++c) {
       if (s_par[c] != v) continue;
       x = s_tok[c];
-      if (x < 0 || x >= V) continue;        // no such token: probability zero
-      const float rx = rest(x);
-      if (s_u[c] * (q ? q[x] : 1.f) < rx) { next = c; break; }
-      if (greedy) continue;                 // one at the maximum stays one there
-      float z = 0.f;
-      for (int i = threadIdx.x; i < V; i += blockDim.x) {
-        const float r = rest(i);
-        z += q ? fmaxf(r - q[i], 0.f) : (i == x ? 0.f : r);
+      if (s_q[c] < 0.f) continue;                      // no such token
+      const float rx = rest(x, s_l[c], s_q[c]);
+      if (s_u[c] * s_q[c] < rx) { next = c; break; }
+      if (greedy) continue;                            // one at the maximum stays one there
+      if (!DRAFT) {
+        // token x leaves; what is left is 1 - r(x) of the remainder (nothing if x is there twice)
+        left = 1.f - rx;
+        if (rx > 0.f && left > 0.f) {
+          if (threadIdx.x == 0) { s_gone[gone] = x; s_mass[gone] = 1.f / left; }
+          __syncthreads();
+          ++gone;
+        }
+        continue;
       }
-      z = block_sum(z, red);
-      if (z > 0.f) { mass[k] = z; gone[k] = x; ++k; }
+      if (c == last) { open = true; break; }
+      float z = 0.f;
+      for (int i0 = lo + int(threadIdx.x); i0 < hi; i0 += kThreads * kUnroll) {
+        float l[kUnroll], qi[kUnroll];
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) {
+          const int i = i0 + u * kThreads;
+          l[u] = i < hi ? logit(i) : -INFINITY;
+          qi[u] = i < hi ? q[i] : 0.f;
+        }
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) z += fmaxf(rest(i0 + u * kThreads, l[u], qi[u]) - qi[u], 0.f);
+      }
+      z = ex.sum(z);
+      if (z > 0.f) {
+        if (threadIdx.x == 0) s_mass[gone] = 1.f / z;
+        __syncthreads();
+        ++gone;
+      }
     }
-    const float lse = smax + logf(total);
     if (next >= 0) {
-      if (threadIdx.x == 0) {
+      if (threadIdx.x == 0 && rank == 0) {
         path[b * N + steps] = v;
         out_tokens[b * N + steps] = x;
-        logprobs[b * N + steps] = logit<BF16>(row, x) / heat - lse;
+        logprobs[b * N + steps] = logprob(s_l[next]);
       }
       ++steps;
       v = next;
-      __syncthreads();
+      __syncthreads();                                 // s_l, s_q, s_mass are rewritten
       continue;
     }
-    float sc = 0.f;
-    int win = -1;
-    for (int i = threadIdx.x; i < V; i += blockDim.x) {
-      float r = rest(i);
-      if (!(r > 0.f)) continue;
-      if (!greedy) r /= noise[size_t(b) * V + i];
-      if (win < 0 || r > sc) { sc = r; win = i; }
+    int win = best;
+    if (!greedy) {
+      // .x, .y: the draw from the remainder; .z, .w: from the remainder before the last rejection, which stands if
+      // that left nothing
+      float4 w = make_float4(0.f, __int_as_float(-1), 0.f, __int_as_float(-1));
+      for (int i0 = lo + int(threadIdx.x); i0 < hi; i0 += kThreads * kUnroll) {
+        float l[kUnroll], qi[kUnroll], ei[kUnroll];
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) {
+          const int i = i0 + u * kThreads;
+          l[u] = i < hi ? logit(i) : -INFINITY;
+          qi[u] = DRAFT && i < hi ? q[i] : 0.f;
+          ei[u] = i < hi ? e[i] : 1.f;
+        }
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) {
+          const int i = i0 + u * kThreads;
+          const float r0 = rest(i, l[u], qi[u]), r1 = DRAFT && open ? fmaxf(r0 - qi[u], 0.f) : r0;
+          const float f = 1.f / ei[u];
+          if (r1 > 0.f && (__float_as_int(w.y) < 0 || r1 * f > w.x)) { w.x = r1 * f; w.y = __int_as_float(i); }
+          if (DRAFT && r0 > 0.f && (__float_as_int(w.w) < 0 || r0 * f > w.z)) { w.z = r0 * f; w.w = __int_as_float(i); }
+        }
+      }
+      w = ex.best2(w);
+      win = __float_as_int(w.y);
+      if (DRAFT && win < 0) win = __float_as_int(w.w);
     }
-    __syncthreads();
-    block_argmax(sc, win, red, redi);
-    if (threadIdx.x == 0) {
+    if (threadIdx.x == 0 && rank == 0) {
       path[b * N + steps] = v;
       out_tokens[b * N + steps] = win;
-      logprobs[b * N + steps] = win >= 0 ? logit<BF16>(row, win) / heat - lse : -INFINITY;
+      logprobs[b * N + steps] = win >= 0 ? logprob(logit(win)) : -INFINITY;
       n_accepted[b] = steps;
     }
     return;
@@ -171,9 +301,30 @@ cudaError_t tree_verify(const void* logits, bool bf16, int64_t ld, int V, const 
                         const float* temperature, const float* draft, int* path, int* n_accepted, int* out_tokens,
                         float* logprobs, cudaStream_t s) {
   if (B == 0) return cudaSuccess;
-  auto f = bf16 ? tree::tree_verify_kernel<true> : tree::tree_verify_kernel<false>;
-  return launch_k(f, dim3(B), 1024, 0, s, logits, ld, V, tokens, cu, parent, N, uniforms, noise, temperature, draft,
-                  path, n_accepted, out_tokens, logprobs);
+  auto f = bf16 ? (draft ? tree::tree_verify_kernel<true, true> : tree::tree_verify_kernel<true, false>)
+                : (draft ? tree::tree_verify_kernel<false, true> : tree::tree_verify_kernel<false, false>);
+  // CTAs per request: as many as keep all requests on the device at once (two CTAs per SM), each with a thousand
+  // tokens or more
+  int dev = 0, sms = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  if (e != cudaSuccess) return e;
+  int c = 1;
+  while (c < tree::kMaxCluster && int64_t(B) * c * 2 <= 2 * sms && V / (2 * c) >= 1024) c *= 2;
+  if (c > 8 && (e = cudaFuncSetAttribute(f, cudaFuncAttributeNonPortableClusterSizeAllowed, 1)) != cudaSuccess) return e;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = c; attr[1].val.clusterDim.y = 1; attr[1].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(unsigned(B) * c);
+  cfg.blockDim = dim3(tree::kThreads);
+  cfg.stream = s;
+  cfg.attrs = pdl_enabled() ? attr : attr + 1;
+  cfg.numAttrs = pdl_enabled() ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, f, logits, ld, V, tokens, cu, parent, N, uniforms, noise, temperature, draft, B,
+                            path, n_accepted, out_tokens, logprobs);
 }
 
 cudaError_t tree_commit(const int64_t* caches, int n, int max_row, bool wide, const TreeLayout& lay, int N, const int* path,
