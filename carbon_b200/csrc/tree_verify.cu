@@ -19,83 +19,66 @@ CB_DEVICE float ex2v(float x) {
   return y;
 }
 
-// One row slice's statistics: maximum, its lowest index, sum of 2^((l - max) k).
-struct Stat {
-  float m, s;
-  int i;
-  CB_DEVICE void join(const Stat& o, float k) {
-    if (o.i < 0) return;
-    if (i < 0) { *this = o; return; }
-    const float t = fmaxf(m, o.m), ref = t == -INFINITY ? 0.f : t;
-    s = s * ex2v((m - ref) * k) + o.s * ex2v((o.m - ref) * k);
-    if (o.m > m || (o.m == m && o.i < i)) i = o.i;
-    m = t;
-  }
-};
-
 // Reductions over the threads of all CTAs of the cluster; every thread gets the result.  A CTA's value goes to every
 // CTA's slot array through distributed shared memory; two arrays alternate, so that one exchange's slots are read
-// before the next but one writes them.
+// before the next but one writes them.  WARP reduces a float4 over the first `w` lanes of a warp (w a power of two).
 struct Exchange {
   float4 (*slots)[kMaxCluster];     // [2][kMaxCluster]
   float4* warps;                    // [kThreads / 32]
   int n, rank, turn;
-  // value of the block (in all threads of warp 0) -> all CTAs
-  CB_DEVICE void all(float4 v) {
-    const int t = turn & 1;
-    if (n == 1) {
-      if (threadIdx.x == 0) slots[t][0] = v;
-      __syncthreads();
-    } else {
-      if (threadIdx.x < uint32_t(n))
-        st_cluster_v4(mapa_shared(smem_u32(&slots[t][rank]), threadIdx.x), __float_as_uint(v.x), __float_as_uint(v.y),
-                      __float_as_uint(v.z), __float_as_uint(v.w));
-      cluster_sync();
-    }
-  }
-  template <typename F>
-  CB_DEVICE float4 reduce(float4 v, F join) {
+  template <typename WARP>
+  CB_DEVICE float4 reduce(float4 v, WARP over) {
     const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
-#pragma unroll
-    for (int o = 16; o; o >>= 1)
-      join(v, make_float4(__shfl_xor_sync(~0u, v.x, o), __shfl_xor_sync(~0u, v.y, o), __shfl_xor_sync(~0u, v.z, o),
-                          __shfl_xor_sync(~0u, v.w, o)));
+    v = over(v, 32);
     if (lane == 0) warps[wid] = v;
     __syncthreads();
-    if (wid == 0) {
-      v = warps[lane & (kThreads / 32 - 1)];
-#pragma unroll
-      for (int o = kThreads / 64; o; o >>= 1)
-        join(v, make_float4(__shfl_xor_sync(~0u, v.x, o), __shfl_xor_sync(~0u, v.y, o), __shfl_xor_sync(~0u, v.z, o),
-                            __shfl_xor_sync(~0u, v.w, o)));
-    }
-    all(v);
     const int t = turn++ & 1;
-    v = slots[t][0];
-    for (int c = 1; c < n; ++c) join(v, slots[t][c]);
-    return v;
+    if (wid == 0) {
+      v = over(warps[lane & (kThreads / 32 - 1)], kThreads / 32);
+      if (n == 1) {
+        if (lane == 0) slots[t][0] = v;
+      } else if (lane < n) {
+        st_cluster_v4(mapa_shared(smem_u32(&slots[t][rank]), lane), __float_as_uint(v.x), __float_as_uint(v.y),
+                      __float_as_uint(v.z), __float_as_uint(v.w));
+      }
+    }
+    if (n == 1) __syncthreads();
+    else cluster_sync();
+    v = slots[t][lane & (n - 1)];
+    return n == 1 ? v : over(v, n);
   }
-  CB_DEVICE Stat stat(const Stat& a, float k) {
-    const float4 r = reduce(make_float4(a.m, a.s, __int_as_float(a.i), 0.f), [&](float4& x, const float4& y) {
-      Stat p{x.x, x.y, __float_as_int(x.z)};
-      p.join(Stat{y.x, y.y, __float_as_int(y.z)}, k);
-      x = make_float4(p.m, p.s, __int_as_float(p.i), 0.f);
+  // (maximum, sum of 2^((l - maximum) k))
+  CB_DEVICE float2 stat(float m, float s, float k) {
+    const float4 r = reduce(make_float4(m, s, 0.f, 0.f), [&](float4 v, int w) {
+      float top = v.x;
+      for (int o = w >> 1; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
+      float sum = v.y * ex2v((v.x - (top == -INFINITY ? 0.f : top)) * k);
+      for (int o = w >> 1; o; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
+      return make_float4(top, sum, 0.f, 0.f);
     });
-    return Stat{r.x, r.y, __float_as_int(r.z)};
+    return make_float2(r.x, r.y);
   }
-  // maxima of two scores at once, lowest index among equals (index -1: none)
+  // maxima of the scores .x and .z and their lowest indices .y, .w (-1: none)
   CB_DEVICE float4 best2(float4 a) {
-    return reduce(a, [](float4& x, const float4& y) {
-      auto take = [](float& v, float& i, float ov, float oi) {
-        const int a = __float_as_int(i), b = __float_as_int(oi);
-        if (b >= 0 && (a < 0 || ov > v || (ov == v && b < a))) { v = ov; i = oi; }
+    return reduce(a, [](float4 v, int w) {
+      auto take = [](float& x, float& i, float ox, float oi) {
+        const int p = __float_as_int(i), q = __float_as_int(oi);
+        if (q >= 0 && (p < 0 || ox > x || (ox == x && q < p))) { x = ox; i = oi; }
       };
-      take(x.x, x.y, y.x, y.y);
-      take(x.z, x.w, y.z, y.w);
+      for (int o = w >> 1; o; o >>= 1) {
+        const float4 y = make_float4(__shfl_xor_sync(~0u, v.x, o), __shfl_xor_sync(~0u, v.y, o),
+                                     __shfl_xor_sync(~0u, v.z, o), __shfl_xor_sync(~0u, v.w, o));
+        take(v.x, v.y, y.x, y.y);
+        take(v.z, v.w, y.z, y.w);
+      }
+      return v;
     });
   }
   CB_DEVICE float sum(float a) {
-    return reduce(make_float4(a, 0.f, 0.f, 0.f), [](float4& x, const float4& y) { x.x += y.x; }).x;
+    return reduce(make_float4(a, 0.f, 0.f, 0.f), [](float4 v, int w) {
+      for (int o = w >> 1; o; o >>= 1) v.x += __shfl_xor_sync(~0u, v.x, o);
+      return v;
+    }).x;
   }
 };
 
@@ -103,14 +86,14 @@ struct Exchange {
 // of a token drawn from a distribution one pass over logits and distribution for the remainder's sum (not needed for
 // the last child, whose remainder goes straight into the draw); the end one pass over logits, distribution and noise.
 template <bool BF16, bool DRAFT>
-__global__ void __launch_bounds__(kThreads) tree_verify_kernel(
+__global__ void __launch_bounds__(kThreads, 2) tree_verify_kernel(
     const void* __restrict__ logits, int64_t ld, int V, const int* __restrict__ tokens, const int* __restrict__ cu,
     const int* __restrict__ parent, int N, const float* __restrict__ uniforms, const float* __restrict__ noise,
     const float* __restrict__ temperature, const float* __restrict__ draft, int clusters, int* __restrict__ path,
     int* __restrict__ n_accepted, int* __restrict__ out_tokens, float* __restrict__ logprobs) {
   pdl_entry();
   __shared__ float4 sh_slots[2][kMaxCluster], sh_warps[kThreads / 32];
-  __shared__ int s_tok[kNodes], s_par[kNodes], s_gone[kNodes];
+  __shared__ int s_tok[kNodes], s_par[kNodes], s_child[kNodes], s_sib[kNodes], s_gone[kNodes];
   __shared__ float s_u[kNodes], s_l[kNodes], s_q[kNodes], s_mass[kNodes];
   const int n_cta = gridDim.x / clusters;
   const int rank = n_cta == 1 ? 0 : int(cluster_ctarank()), b = blockIdx.x / n_cta;
@@ -124,101 +107,124 @@ __global__ void __launch_bounds__(kThreads) tree_verify_kernel(
     }
     if (i < n) { s_tok[i] = tokens[t0 + i]; s_par[i] = parent[t0 + i]; s_u[i] = uniforms[t0 + i]; }
   }
+  const float T = temperature[b];
   if (n_cta > 1) cluster_sync();                       // every CTA runs before any remote store
   else __syncthreads();
   if (n <= 0) {
     if (threadIdx.x == 0 && rank == 0) n_accepted[b] = -1;
     return;
   }
-  const float T = temperature[b];
+  if (int(threadIdx.x) < n) {                          // first child and next sibling of every node (-1: none)
+    const int me = threadIdx.x, up = s_par[me];
+    int child = -1, sib = -1;
+    for (int j = n - 1; j > me; --j) {
+      if (s_par[j] == me) child = j;
+      if (s_par[j] == up) sib = j;
+    }
+    s_child[me] = child;
+    s_sib[me] = sib;
+  }
+  __syncthreads();
   const bool greedy = !(T > 0.f);
   const float k = greedy ? kLog2e : kLog2e / T;        // p = 2^((l - max) k) / total
   const int per = (V + n_cta - 1) / n_cta, lo = rank * per, hi = min(V, lo + per);
+  const float* e = noise + size_t(b) * V;
   int v = 0, steps = 0;
   while (true) {
     const char* rowp = reinterpret_cast<const char*>(logits) + (size_t(t0 + v) * ld) * (BF16 ? 2 : 4);
     const float* q = DRAFT ? draft + size_t(t0 + v) * V : nullptr;
-    const float* e = noise + size_t(b) * V;
     auto logit = [&](int i) -> float {
       if constexpr (BF16) return __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(rowp)[i]);
       else return reinterpret_cast<const float*>(rowp)[i];
     };
     // the children's logits and draft probabilities, read while the pass runs
-    int last = -1;                                     // the last child
-    for (int c = v + 1; c < n; ++c)
-      if (s_par[c] == v) last = c;
     if (int(threadIdx.x) < n && s_par[threadIdx.x] == v) {
       const int x = s_tok[threadIdx.x];
       const bool in = x >= 0 && x < V;
       s_l[threadIdx.x] = in ? logit(x) : -INFINITY;
       s_q[threadIdx.x] = in ? (DRAFT ? q[x] : 1.f) : -1.f;      // no such token: never accepted
     }
-    Stat st{-INFINITY, 0.f, -1};
+    float m = -INFINITY, s = 0.f;
+    int at = -1;
     for (int i0 = lo + int(threadIdx.x); i0 < hi; i0 += kThreads * kUnroll) {
-      float x[kUnroll];
+      float x[kUnroll], top = m;
 #pragma unroll
       for (int u = 0; u < kUnroll; ++u) x[u] = i0 + u * kThreads < hi ? logit(i0 + u * kThreads) : -INFINITY;
-      float m = st.m;
-      int at = st.i < 0 ? i0 : st.i;
+      if (greedy) {
+        if (at < 0) at = i0;
 #pragma unroll
-      for (int u = 0; u < kUnroll; ++u)
-        if (x[u] > m) { m = x[u]; at = i0 + u * kThreads; }
-      const float ref = m == -INFINITY ? 0.f : m;
-      float s = st.s * ex2v((st.m - ref) * k);
+        for (int u = 0; u < kUnroll; ++u)
+          if (x[u] > top) { top = x[u]; at = i0 + u * kThreads; }
+      } else {
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) top = fmaxf(top, x[u]);
+      }
+      const float ref = top == -INFINITY ? 0.f : top;
+      s *= ex2v((m - ref) * k);
 #pragma unroll
       for (int u = 0; u < kUnroll; ++u) s += ex2v((x[u] - ref) * k);
-      st = Stat{m, s, at};
+      m = top;
     }
-    st = ex.stat(st, k);
-    const float ref = st.m == -INFINITY ? 0.f : st.m, total = st.s;
+    const float mine = m;
+    const float2 st = ex.stat(m, s, k);
+    const float ref = st.x == -INFINITY ? 0.f : st.x, total = st.y;
     const float inv = total > 0.f ? 1.f / total : (total == total ? 0.f : total);
-    const int best = total > 0.f ? st.i : -1;
+    int best = -1;                                     // greedy: the lowest-index maximum
+    if (greedy) {
+      best = __float_as_int(ex.best2(make_float4(mine, __int_as_float(at), 0.f, __int_as_float(-1))).y);
+      if (!(total > 0.f)) best = -1;
+    }
     const float lse = log2f(total);
     auto logprob = [&](float l) { return ((l - ref) * k - lse) * 0.6931471805599453f; };
     int gone = 0;                                      // rejections that changed the remainder
-    // remainder of token i with logit l after them
-    auto rest = [&](int i, float l, float qi) -> float {
-      if (greedy) return i == best ? 1.f : 0.f;
-      float r = ex2v((l - ref) * k) * inv;
-      for (int j = 0; j < gone; ++j) r = DRAFT ? fmaxf(r - qi, 0.f) * s_mass[j] : (s_gone[j] == i ? 0.f : r * s_mass[j]);
-      return r;
+    // remainder of the tokens i0, i0 + kThreads, ... with logits r[] after them
+    auto rest = [&](float* r, const float* qi, int i0, int cnt) {
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u)
+        if (u < cnt) r[u] = ex2v((r[u] - ref) * k) * inv;
+      for (int j = 0; j < gone; ++j) {
+        const float f = s_mass[j];
+        const int x = DRAFT ? 0 : s_gone[j];
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u)
+          if (u < cnt) r[u] = DRAFT ? fmaxf(r[u] - qi[u], 0.f) * f : (x == i0 + u * kThreads ? 0.f : r[u] * f);
+      }
     };
     int next = -1, x = -1;
     bool open = false;                                 // the last child's rejection goes into the draw
-    float left = 1.f;                                  // mass of the certain proposals' remainder
-    for (int c = v + 1; c <= last && next < 0; ++c) {
-      if (s_par[c] != v) continue;
+    for (int c = s_child[v]; c >= 0; c = s_sib[c]) {
       x = s_tok[c];
-      if (s_q[c] < 0.f) continue;                      // no such token
-      const float rx = rest(x, s_l[c], s_q[c]);
-      if (s_u[c] * s_q[c] < rx) { next = c; break; }
+      const float qx = s_q[c];
+      if (qx < 0.f) continue;                          // no such token
+      float rx = s_l[c];
+      if (greedy) rx = x == best ? 1.f : 0.f;
+      else rest(&rx, &qx, x, 1);
+      if (s_u[c] * qx < rx) { next = c; break; }
       if (greedy) continue;                            // one at the maximum stays one there
-      if (!DRAFT) {
-        // token x leaves; what is left is 1 - r(x) of the remainder (nothing if x is there twice)
-        left = 1.f - rx;
-        if (rx > 0.f && left > 0.f) {
-          if (threadIdx.x == 0) { s_gone[gone] = x; s_mass[gone] = 1.f / left; }
-          __syncthreads();
-          ++gone;
-        }
-        continue;
-      }
-      if (c == last) { open = true; break; }
       float z = 0.f;
-      for (int i0 = lo + int(threadIdx.x); i0 < hi; i0 += kThreads * kUnroll) {
-        float l[kUnroll], qi[kUnroll];
+      if (!DRAFT) {
+        // token x leaves: 1 - r(x) of the remainder is left (all of it if x has left before)
+        z = rx > 0.f ? 1.f - rx : 0.f;
+      } else if (s_sib[c] < 0) {
+        open = true;
+        break;
+      } else {
+        for (int i0 = lo + int(threadIdx.x); i0 < hi; i0 += kThreads * kUnroll) {
+          float r[kUnroll], qi[kUnroll];
 #pragma unroll
-        for (int u = 0; u < kUnroll; ++u) {
-          const int i = i0 + u * kThreads;
-          l[u] = i < hi ? logit(i) : -INFINITY;
-          qi[u] = i < hi ? q[i] : 0.f;
+          for (int u = 0; u < kUnroll; ++u) {
+            const int i = i0 + u * kThreads;
+            r[u] = i < hi ? logit(i) : -INFINITY;
+            qi[u] = i < hi ? q[i] : 0.f;
+          }
+          rest(r, qi, i0, kUnroll);
+#pragma unroll
+          for (int u = 0; u < kUnroll; ++u) z += fmaxf(r[u] - qi[u], 0.f);
         }
-#pragma unroll
-        for (int u = 0; u < kUnroll; ++u) z += fmaxf(rest(i0 + u * kThreads, l[u], qi[u]) - qi[u], 0.f);
+        z = ex.sum(z);
       }
-      z = ex.sum(z);
       if (z > 0.f) {
-        if (threadIdx.x == 0) s_mass[gone] = 1.f / z;
+        if (threadIdx.x == 0) { s_gone[gone] = x; s_mass[gone] = 1.f / z; }
         __syncthreads();
         ++gone;
       }
@@ -236,28 +242,29 @@ __global__ void __launch_bounds__(kThreads) tree_verify_kernel(
     }
     int win = best;
     if (!greedy) {
-      // .x, .y: the draw from the remainder; .z, .w: from the remainder before the last rejection, which stands if
-      // that left nothing
-      float4 w = make_float4(0.f, __int_as_float(-1), 0.f, __int_as_float(-1));
+      // The draw: r / e is compared as r * e' > r' * e.  Second result: the draw from the remainder before the last
+      // rejection, which stands if that left nothing.
+      float r1 = 0.f, e1 = 1.f, r0 = 0.f, e0 = 1.f;
+      int w1 = -1, w0 = -1;
       for (int i0 = lo + int(threadIdx.x); i0 < hi; i0 += kThreads * kUnroll) {
-        float l[kUnroll], qi[kUnroll], ei[kUnroll];
+        float r[kUnroll], qi[kUnroll], ei[kUnroll];
 #pragma unroll
         for (int u = 0; u < kUnroll; ++u) {
           const int i = i0 + u * kThreads;
-          l[u] = i < hi ? logit(i) : -INFINITY;
+          r[u] = i < hi ? logit(i) : -INFINITY;
           qi[u] = DRAFT && i < hi ? q[i] : 0.f;
           ei[u] = i < hi ? e[i] : 1.f;
         }
+        rest(r, qi, i0, kUnroll);
 #pragma unroll
         for (int u = 0; u < kUnroll; ++u) {
           const int i = i0 + u * kThreads;
-          const float r0 = rest(i, l[u], qi[u]), r1 = DRAFT && open ? fmaxf(r0 - qi[u], 0.f) : r0;
-          const float f = 1.f / ei[u];
-          if (r1 > 0.f && (__float_as_int(w.y) < 0 || r1 * f > w.x)) { w.x = r1 * f; w.y = __int_as_float(i); }
-          if (DRAFT && r0 > 0.f && (__float_as_int(w.w) < 0 || r0 * f > w.z)) { w.z = r0 * f; w.w = __int_as_float(i); }
+          if (DRAFT && r[u] * e0 > r0 * ei[u]) { r0 = r[u]; e0 = ei[u]; w0 = i; }
+          const float d = DRAFT && open ? fmaxf(r[u] - qi[u], 0.f) : r[u];
+          if (d * e1 > r1 * ei[u]) { r1 = d; e1 = ei[u]; w1 = i; }
         }
       }
-      w = ex.best2(w);
+      const float4 w = ex.best2(make_float4(r1 / e1, __int_as_float(w1), r0 / e0, __int_as_float(w0)));
       win = __float_as_int(w.y);
       if (DRAFT && win < 0) win = __float_as_int(w.w);
     }
