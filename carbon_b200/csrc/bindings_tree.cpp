@@ -155,17 +155,21 @@ int tree_mla(const Tensor& q, const Tensor& kv, const Tensor& cu, const Tensor& 
                       reinterpret_cast<float*>(ws + off[3]), ptr<int>(status), out.data_ptr(), stream());
 }
 
-// out: int32 [B (2 N + 1)] = path, tokens, n_accepted
-int tree_verify(const Tensor& logits, const Tensor& tokens, const Tensor& cu, const Tensor& parent, int64_t N,
-                const Tensor& uniforms, const Tensor& noise, const Tensor& temperature, const OptTensor& draft,
-                const Tensor& out, const Tensor& logprobs) {
+// out: int32 [B (2 N + 1)] = path [B, N], n_accepted [B], tokens [B, N], returned as views
+std::tuple<int, Tensor, Tensor, Tensor> tree_verify(const Tensor& logits, const Tensor& tokens, const Tensor& cu,
+                                                    const Tensor& parent, int64_t N, const Tensor& uniforms,
+                                                    const Tensor& noise, const Tensor& temperature,
+                                                    const OptTensor& draft, const Tensor& out,
+                                                    const Tensor& logprobs) {
   c10::cuda::CUDAGuard g(logits.device());
   const int64_t B = cu.numel() - 1;
   int* o = ptr<int>(out);
-  return cb::tree_verify(logits.data_ptr(), logits.scalar_type() == at::kBFloat16, logits.stride(0),
-                         int(logits.size(1)), ptr<int>(tokens), ptr<int>(cu), ptr<int>(parent), int(B), int(N),
-                         ptr<float>(uniforms), ptr<float>(noise), ptr<float>(temperature), ptr<float>(draft), o,
-                         o + 2 * B * N, o + B * N, ptr<float>(logprobs), stream());
+  const int e = cb::tree_verify(logits.data_ptr(), logits.scalar_type() == at::kBFloat16, logits.stride(0),
+                                int(logits.size(1)), ptr<int>(tokens), ptr<int>(cu), ptr<int>(parent), int(B), int(N),
+                                ptr<float>(uniforms), ptr<float>(noise), ptr<float>(temperature), ptr<float>(draft),
+                                o, o + B * N, o + B * (N + 1), ptr<float>(logprobs), stream());
+  return {e, out.as_strided({B, N}, {N, 1}, 0), out.as_strided({B}, {1}, B * N),
+          out.as_strided({B, N}, {N, 1}, B * (N + 1))};
 }
 
 int tree_commit(const Tensor& caches, int64_t max_row, bool wide, const Tensor& cu, const Tensor& ctx,

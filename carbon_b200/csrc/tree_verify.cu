@@ -10,7 +10,7 @@
 namespace cb {
 namespace tree {
 
-constexpr int kNodes = 64, kThreads = 512, kUnroll = 8, kMaxCluster = 16;
+constexpr int kNodes = 64, kThreads = 512, kUnroll = 8, kWide = 16, kMaxCluster = 16;
 constexpr float kLog2e = 1.4426950408889634f;
 
 CB_DEVICE float ex2v(float x) {
@@ -146,23 +146,23 @@ __global__ void __launch_bounds__(kThreads, 2) tree_verify_kernel(
     }
     float m = -INFINITY, s = 0.f;
     int at = -1;
-    for (int i0 = lo + int(threadIdx.x); i0 < hi; i0 += kThreads * kUnroll) {
-      float x[kUnroll], top = m;
+    for (int i0 = lo + int(threadIdx.x); i0 < hi; i0 += kThreads * kWide) {
+      float x[kWide], top = m;
 #pragma unroll
-      for (int u = 0; u < kUnroll; ++u) x[u] = i0 + u * kThreads < hi ? logit(i0 + u * kThreads) : -INFINITY;
+      for (int u = 0; u < kWide; ++u) x[u] = i0 + u * kThreads < hi ? logit(i0 + u * kThreads) : -INFINITY;
       if (greedy) {
         if (at < 0) at = i0;
 #pragma unroll
-        for (int u = 0; u < kUnroll; ++u)
+        for (int u = 0; u < kWide; ++u)
           if (x[u] > top) { top = x[u]; at = i0 + u * kThreads; }
       } else {
 #pragma unroll
-        for (int u = 0; u < kUnroll; ++u) top = fmaxf(top, x[u]);
+        for (int u = 0; u < kWide; ++u) top = fmaxf(top, x[u]);
       }
       const float ref = top == -INFINITY ? 0.f : top;
       s *= ex2v((m - ref) * k);
 #pragma unroll
-      for (int u = 0; u < kUnroll; ++u) s += ex2v((x[u] - ref) * k);
+      for (int u = 0; u < kWide; ++u) s += ex2v((x[u] - ref) * k);
       m = top;
     }
     const float mine = m;

@@ -26,6 +26,7 @@ import torch
 from ..ref import ops as R
 from ._ext import ext
 
+_ROW_BYTES = {576: 656, 512: 528}      # an fp8 cache row (ref.ops.latent_fp8_row_bytes)
 MAX_NODES = 64           # nodes of one request's tree: one bit each in a node's mask
 
 
@@ -85,6 +86,7 @@ class TreePlan:
             req += [b] * k
             par += p
             pos += [c + d for d in depth]
+        self._ws = {}
         self.ctx_list, self.tables_list, self.parents_list = [int(c) for c in ctx], page_tables, parents
         self.cu_list, self.pos_list = cu, pos
         self.max_page = max((pg for tab in page_tables for pg in tab), default=-1)
@@ -116,6 +118,21 @@ class TreePlan:
         self.cu, self.ctx, self.req, self.parent, self.pos, self.table = out
         self.table = self.table.view(B, P)
 
+    def _workspace(self, f8: bool, D: int):
+        """(whether every row is staged, byte offsets of the workspace's parts, its size) of an attention call.  Rows
+        that TMA cannot take from the cache as they lie are staged in a dense 16-bit buffer: fp8 rows, and pages that
+        are no multiple of 8 rows (a swizzle group); else only each request's last tiles."""
+        got = self._ws.get((f8, D))
+        if got is None:
+            whole = f8 or self.page_size % 8 != 0
+            parts = self._counts[3]
+            off, end = [], 0
+            for k in (self._counts[5 if whole else 4] * 256 * D, 4 * self.T, parts * 128 * 2048, parts * 128 * 8):
+                off.append(end)
+                end += (k + 255) // 256 * 256
+            got = self._ws[(f8, D)] = (whole, off, end)
+        return got
+
     def check(self) -> None:
         """Raise if a kernel of this plan gave up a wait (reads from the device)."""
         if int(self.status):
@@ -139,9 +156,10 @@ class TreePlan:
                              f"cache holds {slots}")
 
 
-def _need(what: str, t: torch.Tensor, device, dtype) -> None:
-    if t.dtype != dtype or t.device != device or not t.is_contiguous():
-        raise ValueError(f"{what} must be contiguous {dtype} on {device}, got {t.dtype} on {t.device}"
+def _need(what: str, t: torch.Tensor, dev: int, dtype) -> None:
+    """dev: a CUDA device's index."""
+    if t.dtype is not dtype or t.get_device() != dev or not t.is_contiguous():
+        raise ValueError(f"{what} must be contiguous {dtype} on cuda:{dev}, got {t.dtype} on {t.device}"
                          f"{'' if t.is_contiguous() else ' (not contiguous)'}")
 
 
@@ -162,7 +180,7 @@ def tree_mla(q: torch.Tensor, kv: torch.Tensor, plan: TreePlan, scale: float, d_
     plan._check("tree_mla", kv.shape[0])
     if not scale > 0:
         raise ValueError(f"tree_mla: scale must be positive, got {scale}")
-    if sink is not None and tuple(sink.shape) != (H,):
+    if sink is not None and sink.shape != (H,):
         raise ValueError(f"tree_mla: sink has shape {tuple(sink.shape)}, expected {(H,)}")
     if q.is_cuda:
         if D not in (576, 512) or d_latent != 512:
@@ -170,26 +188,20 @@ def tree_mla(q: torch.Tensor, kv: torch.Tensor, plan: TreePlan, scale: float, d_
                                "d_latent=512")
         if H != plan.n_heads:
             raise ValueError(f"tree_mla: q has {H} heads, the plan was made for {plan.n_heads}")
-        if q.device != plan.device:
+        dev = plan.device.index
+        if q.get_device() != dev:
             raise ValueError(f"tree_mla: q is on {q.device}, the plan on {plan.device}")
-        _need("tree_mla: kv", kv, q.device, torch.uint8 if f8 else torch.bfloat16)
-        if kv.dim() != 2 or kv.shape[1] != (R.latent_fp8_row_bytes(512, 64, D == 576) if f8 else D):
+        _need("tree_mla: kv", kv, dev, torch.uint8 if f8 else torch.bfloat16)
+        if kv.dim() != 2 or kv.shape[1] != (_ROW_BYTES[D] if f8 else D):
             raise ValueError(f"tree_mla: kv of shape {tuple(kv.shape)} does not hold rows for width {D}")
-        qk = q.to(torch.float16 if f8 else torch.bfloat16).contiguous()
+        want = torch.float16 if f8 else torch.bfloat16
+        qk = q if q.dtype is want and q.is_contiguous() else q.to(want).contiguous()
         if sink is not None:
-            sink = sink.to(q.device, torch.float32).contiguous()
+            _need("tree_mla: sink", sink, dev, torch.float32)
         out = torch.empty(T, H, 512, dtype=torch.bfloat16, device=q.device)
         if T:
-            # rows that TMA cannot take from the cache as they lie are staged: fp8 rows, pages that are no multiple of
-            # 8 rows (a swizzle group); else only each request's last tiles
-            whole = f8 or plan.page_size % 8 != 0
-            parts = plan._counts[3]
-            sizes = (plan._counts[5 if whole else 4] * 256 * D, 4 * T, parts * 128 * 2048, parts * 128 * 8)
-            off, end = [], 0
-            for k in sizes:
-                off.append(end)
-                end += (k + 255) // 256 * 256
-            buf = torch.empty(end, dtype=torch.uint8, device=q.device)
+            whole, off, size = plan._workspace(f8, D)
+            buf = torch.empty(size, dtype=torch.uint8, device=q.device)
             _launched(ext().tree_mla(qk, kv, plan.cu, plan.ctx, plan.table, plan.mask, plan.page_size, whole,
                                      plan._work, plan._counts, buf, off, float(scale), sink, plan.status, out),
                       "tree_mla")
@@ -230,27 +242,27 @@ def tree_verify(logits: torch.Tensor, tokens: torch.Tensor, plan: TreePlan, unif
     for name, t, shape in (("logits", logits, (T, V)), ("tokens", tokens, (T,)), ("uniforms", uniforms, (T,)),
                            ("noise", noise, (B, V)), ("temperature", temperature, (B,)),
                            ("draft_probs", draft_probs, (T, V))):
-        if t is not None and tuple(t.shape) != shape:
+        if t is not None and t.shape != shape:
             raise ValueError(f"tree_verify: {name} has shape {tuple(t.shape)}, expected {shape}")
     N = plan.N
     if logits.is_cuda:
-        dev = plan.device
-        if logits.device != dev or logits.dtype not in (torch.float32, torch.bfloat16) or not 0 < V < 1 << 31 or (
+        dev = plan.device.index
+        if logits.get_device() != dev or logits.dtype not in (torch.float32, torch.bfloat16) or not 0 < V < 1 << 31 or (
                 T and logits.stride(1) != 1):
-            raise ValueError(f"tree_verify: logits must be fp32 or bf16 on {dev} with a unit column stride, got "
-                             f"{logits.dtype} on {logits.device}, strides {logits.stride()}")
+            raise ValueError(f"tree_verify: logits must be fp32 or bf16 on {plan.device} with a unit column stride, "
+                             f"got {logits.dtype} on {logits.device}, strides {logits.stride()}")
         _need("tree_verify: tokens", tokens, dev, torch.int32)
         _need("tree_verify: uniforms", uniforms, dev, torch.float32)
         _need("tree_verify: noise", noise, dev, torch.float32)
         _need("tree_verify: temperature", temperature, dev, torch.float32)
         if draft_probs is not None:
             _need("tree_verify: draft_probs", draft_probs, dev, torch.float32)
-        out = torch.empty(B * (2 * N + 1), dtype=torch.int32, device=dev)
-        lp = torch.empty(B, N, dtype=torch.float32, device=dev)
-        if B:
-            _launched(ext().tree_verify(logits, tokens, plan.cu, plan.parent, N, uniforms, noise, temperature,
-                                        draft_probs, out, lp), "tree_verify")
-        return TreeVerdict(out[:B * N].view(B, N), out[2 * B * N:], out[B * N:2 * B * N].view(B, N), lp)
+        out = torch.empty(B * (2 * N + 1), dtype=torch.int32, device=logits.device)
+        lp = torch.empty(B, N, dtype=torch.float32, device=logits.device)
+        code, path, n, toks = ext().tree_verify(logits, tokens, plan.cu, plan.parent, N, uniforms, noise, temperature,
+                                                draft_probs, out, lp)
+        _launched(code, "tree_verify")
+        return TreeVerdict(path, n, toks, lp)
     v = TreeVerdict(torch.full((B, N), -1, dtype=torch.int32), torch.full((B,), -1, dtype=torch.int32),
                     torch.full((B, N), -1, dtype=torch.int32), torch.zeros(B, N))
     for b in range(B):
@@ -294,15 +306,15 @@ def tree_commit(rows: CacheRows, plan: TreePlan, path: torch.Tensor, n_accepted:
     """Move the accepted branch's cache rows behind the context, in place: for k = 1 .. n_accepted[b], the row of node
     path[b, k] goes to position ctx[b] + k (node k's old row).  path [B, N] and n_accepted [B] as ``tree_verify``
     returns them."""
-    if tuple(path.shape) != (plan.B, plan.N) or tuple(n_accepted.shape) != (plan.B,):
+    if path.shape != (plan.B, plan.N) or n_accepted.shape != (plan.B,):
         raise ValueError(f"tree_commit: path {tuple(path.shape)} and n_accepted {tuple(n_accepted.shape)}, expected "
                          f"{(plan.B, plan.N)} and {(plan.B,)}")
     plan._check("tree_commit", rows.slots)
     if rows.device.type == "cuda":
         if rows.device != plan.device:
             raise ValueError(f"tree_commit: the caches are on {rows.device}, the plan on {plan.device}")
-        _need("tree_commit: path", path, rows.device, torch.int32)
-        _need("tree_commit: n_accepted", n_accepted, rows.device, torch.int32)
+        _need("tree_commit: path", path, plan.device.index, torch.int32)
+        _need("tree_commit: n_accepted", n_accepted, plan.device.index, torch.int32)
         if plan.N > 1:
             _launched(ext().tree_commit(rows.table, rows.max_row, rows.wide, plan.cu, plan.ctx, plan.table,
                                         plan.page_size, path, n_accepted), "tree_commit")
