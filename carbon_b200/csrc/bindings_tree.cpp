@@ -33,12 +33,15 @@ cb::TreeLayout layout(const Tensor& cu, const Tensor& ctx, const Tensor& table, 
 // share grows a little until no piece comes out shorter than kPiece.  The row tiles of a request are handed out one
 // after the other, so they run at about the same time and read its keys from L2.  kOver: cost of an item's start and
 // end in key tiles.
-// -> int32 tensor: first [clusters + 1], items [*, 5], merges [*, 4], (even offset) staged blocks of the tail mode
-// [*, 2], of the all mode [*, 2], first block per request of either [B] [B]; and the counts
+// -> int32 tensor (16-byte aligned parts): first [clusters + 1], items [*, 8], merges [*, 6], whole key tiles (request,
+// tile) [*, 2], first of them per request [B]; and the counts of CTA pairs, items, merges, partial results, whole key
+// tiles and key tiles over all items
 std::tuple<Tensor, std::vector<int64_t>> tree_schedule(const std::vector<int64_t>& n, const std::vector<int64_t>& ctx,
                                                        int64_t H, int64_t clusters) {
   constexpr int64_t kTile = 128, kOver = 2, kPiece = 2;
   const int64_t B = int64_t(n.size());
+  std::vector<int64_t> cu(B + 1, 0);
+  for (int64_t b = 0; b < B; ++b) cu[b + 1] = cu[b] + n[b];
   struct Row { int64_t b, row, tiles; };
   std::vector<Row> rows;
   int64_t total = 0;
@@ -70,13 +73,13 @@ std::tuple<Tensor, std::vector<int64_t>> tree_schedule(const std::vector<int64_t
         const int64_t take = force || rest < room + std::min(kPiece, share / 16 + 1) ? rest : room;
         auto& list = lists[ld.second];
         pieces.push_back({ld.second, list.size()});
-        list.push_back({int(r.b), int(r.row), int(at), int(take), -1});
+        list.push_back({int(r.b), int(r.row), int(at), int(take), -1, int(ctx[r.b]), int(cu[r.b]), int(n[r.b])});
         heap.push({ld.first + take + kOver, ld.second});
         at += take;
       }
       if (pieces.size() > 1) {
         for (auto& [c, i] : pieces) lists[c][i].part = int(parts++);
-        merges.push_back({int(r.b), int(r.row), int(first_part), int(pieces.size())});
+        merges.push_back({int(r.row), int(first_part), int(pieces.size()), int(cu[r.b]), int(n[r.b] * H), 0});
       }
     }
     return true;
@@ -84,75 +87,59 @@ std::tuple<Tensor, std::vector<int64_t>> tree_schedule(const std::vector<int64_t
   int64_t share = std::max((total + clusters - 1) / clusters, kPiece + kOver);
   int tries = 0;
   while (!assign(share, ++tries > 60)) share += std::max<int64_t>(1, share / 40);
-  int64_t used = 0, n_items = 0, n_tail = 0, n_all = 0;
+  int64_t used = 0, n_items = 0;
   for (auto& l : lists) { used += !l.empty(); n_items += int64_t(l.size()); }
   std::stable_sort(lists.begin(), lists.end(), [](const auto& x, const auto& y) { return !x.empty() && y.empty(); });
-  for (int64_t b = 0; b < B; ++b) {
-    if (!n[b]) continue;
-    const int64_t tiles = (ctx[b] + n[b] + kTile - 1) / kTile;
-    n_tail += tiles - ctx[b] / kTile;
-    n_all += tiles;
-  }
-  int64_t size = used + 1 + n_items * 5 + int64_t(merges.size()) * 4;
-  size += size & 1;
-  auto out = torch::empty({size + 2 * n_tail + 2 * n_all + 2 * B}, torch::kInt32);
+  const int64_t head = (used + 1 + 3) / 4 * 4;
+  int64_t n_stage = 0, work = 0;
+  for (int64_t b = 0; b < B; ++b) n_stage += n[b] ? ctx[b] / kTile : 0;
+  for (const Row& r : rows) work += r.tiles;
+  const int64_t tail = head + n_items * 8 + int64_t(merges.size()) * 6;
+  auto out = torch::empty({(tail + 2 * n_stage + B + 3) / 4 * 4}, torch::kInt32);
   int* o = ptr<int>(out);
-  int* items = o + used + 1;
-  o[0] = 0;
   int at = 0;
-  for (int64_t c = 0; c < used; ++c) {
-    for (const auto& it : lists[c]) std::memcpy(items + 5 * at++, &it, sizeof it);
-    o[c + 1] = at;
+  for (int64_t c = 0; c < head; ++c) {
+    o[c] = at;
+    if (c < used)
+      for (const auto& it : lists[c]) std::memcpy(o + head + 8 * at++, &it, sizeof it);
   }
-  if (!merges.empty()) std::memcpy(items + 5 * n_items, merges.data(), merges.size() * sizeof merges[0]);
-  int* tail = o + size;
-  int* all = tail + 2 * n_tail;
-  int* at_tail = all + 2 * n_all;
-  int* at_all = at_tail + B;
-  int it = 0, ia = 0;
+  if (!merges.empty()) std::memcpy(o + head + 8 * n_items, merges.data(), merges.size() * sizeof merges[0]);
+  int* st = o + tail;
+  int* first = st + 2 * n_stage;
+  int k = 0;
   for (int64_t b = 0; b < B; ++b) {
-    at_tail[b] = it;
-    at_all[b] = ia;
-    if (!n[b]) continue;
-    const int64_t tiles = (ctx[b] + n[b] + kTile - 1) / kTile;
-    for (int64_t t = 0; t < tiles; ++t) {
-      all[2 * ia] = int(b);
-      all[2 * ia++ + 1] = int(t);
-      if (t < ctx[b] / kTile) continue;
-      tail[2 * it] = int(b);
-      tail[2 * it++ + 1] = int(t);
+    first[b] = k;
+    for (int64_t t = 0; n[b] && t < ctx[b] / kTile; ++t, ++k) {
+      st[2 * k] = int(b);
+      st[2 * k + 1] = int(t);
     }
   }
-  return {out, {used, n_items, int64_t(merges.size()), parts, n_tail, n_all, size}};
+  return {out, {used, n_items, int64_t(merges.size()), parts, n_stage, work}};
 }
 
-// work: tree_schedule's tensor on the device, counts its counts; buf: workspace (sizes in tree_mla_workspace's order:
-// staged rows, bad [T], partial outputs, partial (m, l)) at byte offsets off[0..3]
+// work: tree_schedule's tensor on the device, counts its counts; buf: workspace of the partial outputs, then (m, l);
+// staged: workspace of the dense key rows, if they are to be staged
 int tree_mla(const Tensor& q, const Tensor& kv, const Tensor& cu, const Tensor& ctx, const Tensor& table,
-             const Tensor& mask, int64_t page, bool all, const Tensor& work, const std::vector<int64_t>& counts,
-             const Tensor& buf, const std::vector<int64_t>& off, double scale, const OptTensor& sink,
-             const Tensor& status, const Tensor& out) {
+             const Tensor& mask, int64_t page, const Tensor& work, const std::vector<int64_t>& counts,
+             const OptTensor& buf, const OptTensor& staged, double scale, const OptTensor& sink, const Tensor& status,
+             const Tensor& out) {
   c10::cuda::CUDAGuard g(q.device());
-  const int64_t used = counts[0], n_items = counts[1], n_merges = counts[2], n_tail = counts[4], n_all = counts[5];
   const int* w = ptr<int>(work);
-  const int* tail = w + counts[6];
-  const int* every = tail + 2 * n_tail;
-  const int* at = every + 2 * n_all;
+  const int64_t head = (counts[0] + 1 + 3) / 4 * 4;
   cb::TreeWork tw;
   tw.first = w;
-  tw.items = reinterpret_cast<const cb::TreeItem*>(w + used + 1);
-  tw.merges = reinterpret_cast<const cb::TreeMerge*>(w + used + 1 + 5 * n_items);
-  tw.clusters = int(used);
-  tw.n_merges = int(n_merges);
-  tw.n_parts = int(counts[3]);
-  tw.stage = reinterpret_cast<const int2*>(all ? every : tail);
-  tw.stage_at = at + (all ? table.size(0) : 0);
-  tw.n_stage = int(all ? n_all : n_tail);
-  uint8_t* ws = ptr<uint8_t>(buf);
-  return cb::tree_mla(q.data_ptr(), q.size(0), q.size(1), q.size(2), kv.scalar_type() == at::kByte, all, kv.data_ptr(),
+  tw.items = reinterpret_cast<const cb::TreeItem*>(w + head);
+  tw.merges = reinterpret_cast<const cb::TreeMerge*>(w + head + 8 * counts[1]);
+  tw.clusters = int(counts[0]);
+  tw.n_merges = int(counts[2]);
+  const int* st = w + head + 8 * counts[1] + 6 * counts[2];
+  tw.stage = reinterpret_cast<const int2*>(st);
+  tw.stage_at = st + 2 * counts[4];
+  tw.n_stage = int(counts[4]);
+  float* part = ptr<float>(buf);
+  return cb::tree_mla(q.data_ptr(), q.size(0), q.size(1), q.size(2), kv.scalar_type() == at::kByte, kv.data_ptr(),
                       kv.size(0), layout(cu, ctx, table, page), tw, ptr<int64_t>(mask), float(scale), ptr<float>(sink),
-                      ws + off[0], reinterpret_cast<int*>(ws + off[1]), reinterpret_cast<float*>(ws + off[2]),
-                      reinterpret_cast<float*>(ws + off[3]), ptr<int>(status), out.data_ptr(), stream());
+                      part, part ? part + counts[3] * 128 * 512 : nullptr, ptr<void>(staged), ptr<int>(status), out.data_ptr(), stream());
 }
 
 // out: int32 [B (2 N + 1)] = path [B, N], n_accepted [B], tokens [B, N], returned as views

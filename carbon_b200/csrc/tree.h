@@ -16,26 +16,31 @@ struct TreeLayout {
 
 // Work of one attention call, made by tree_schedule: a CTA pair runs the items [first[c], first[c + 1]) one after the
 // other.  An item is one 128-row tile (rows = nodes x heads of one request) over a range of 128-key tiles.
-struct TreeItem { int b, row, tile, n_tiles, part; };      // part: partial-result slot, -1 = the whole row tile
-struct TreeMerge { int b, row, part, n; };                 // row tile whose partial results [part, part + n) are merged
+struct alignas(16) TreeItem {
+  int b, row, tile, n_tiles;
+  int part;                // partial-result slot, -1 = the whole row tile
+  int ctx, c0, n;          // the request's cached tokens, first node row and nodes
+};
+// A row tile whose partial results [part, part + n) are merged; its request's first node row and nodes x heads rows.
+struct alignas(8) TreeMerge { int row, part, n, c0, rows, pad; };
 struct TreeWork {
   const int* first;        // [clusters + 1]
   const TreeItem* items;
   const TreeMerge* merges;
-  int clusters, n_merges, n_parts;
-  // 128-row blocks of the staging buffer: (request, key tile) each; the request's first block is stage_at[b] and its
-  // first staged key tile stage_tile(b): 0 when every row is staged, else ctx / 128
+  int clusters, n_merges;
+  // 128-row blocks of the staging buffer, one per whole key tile before the tree: (request, key tile), and each
+  // request's first block
   const int2* stage;
   const int* stage_at;     // [B]
   int n_stage;
 };
 
-// q [T, H, D] (bf16; fp16 for fp8 rows), kv rows [S, row bytes], mask [T] (bit j: the node sees node j), req [T]
-// -> out [T, H, 512] bf16.  all: every key row is staged (fp8 rows; pages that are no multiple of 8).
-// staged [n_stage * 128, D] 16-bit, bad [T], part_o [n_parts, 128, 512], part_ml [n_parts, 128, 2]: workspaces.
-cudaError_t tree_mla(const void* q, int T, int H, int D, bool f8, bool all, const void* kv, int64_t S,
-                     const TreeLayout& lay, const TreeWork& work, const int64_t* mask, float scale, const float* sink,
-                     void* staged, int* bad, float* part_o, float* part_ml, int* status, void* out, cudaStream_t s);
+// q [T, H, D] (bf16; fp16 for fp8 rows), kv rows [S, row bytes], mask [T] (bit j: the node sees node j)
+// -> out [T, H, 512] bf16.  part_o [parts, 128, 512], part_ml [parts, 128, 2]: workspaces; staged: null, or
+// [n_stage * 128, D] 16-bit, where whole key tiles are first expanded to dense rows.
+cudaError_t tree_mla(const void* q, int T, int H, int D, bool f8, const void* kv, int64_t S, const TreeLayout& lay,
+                     const TreeWork& work, const int64_t* mask, float scale, const float* sink, float* part_o,
+                     float* part_ml, void* staged, int* status, void* out, cudaStream_t s);
 // CTA pairs of the attention kernel that fit on the current device at once
 int tree_mla_clusters();
 

@@ -8,9 +8,10 @@
 // TMEM columns (an M = 128 pair tile keeps the first half of N in lanes 0-63 and the second half in lanes 64-127),
 // which leaves room for two score tiles.  (One CTA with M = 128 rows would need all 512 columns for O.)
 //
-// Three launches: tree_stage_kernel brings the key rows that the tensor core cannot take as they lie in the cache (fp8
-// rows, rows of small pages, and always the last tiles, whose rows end or belong to the tree) into a dense buffer;
-// tree_mla_kernel does the attention; tree_merge_kernel joins row tiles whose keys were split over CTA pairs.
+// Key tiles come into shared memory by TMA where they lie there as the tensor core reads them: whole tiles of bf16 rows
+// in pages of a multiple of 64.  fp8 rows, other pages and each request's last tiles (which end, or belong to the tree)
+// are fed by warps: global memory -> registers -> fp16 / bf16 in the swizzled layout.  tree_merge_kernel joins row tiles
+// whose keys were split over CTA pairs.
 #include <cudaTypedefs.h>
 #include <cuda_fp16.h>
 #include "ptx.cuh"
@@ -26,17 +27,19 @@ constexpr int STAGE = SLOTS * CH;
 constexpr int NST = 2;
 constexpr int TM_O = 0, TM_S = 256;        // TMEM columns: O 256, two score buffers of 64
 constexpr int SM_WARPS = 8;                // softmax warps: two per 32 TMEM lanes, each one half of the score columns
-constexpr int THREADS = 128 + SM_WARPS * 32;
+constexpr int FEED_WARPS = 8;              // eight rows (one swizzle group) of a CTA's 64 keys each
+constexpr int THREADS = 64 + FEED_WARPS * 32 + SM_WARPS * 32;
 constexpr int SMEM_USED = SLOTS * CH + NST * STAGE + CH + 2048 + 256;
 constexpr int SMEM = SMEM_USED + 768;      // 227 KB; the base is 256-byte aligned at least (checked by the kernel)
 constexpr float kRescale = 8.f;            // O is rescaled when the running maximum grows by more than 2^8
 
+enum { FEED, PAGED, STAGED };
 struct Params {
   TreeLayout lay;
   TreeWork work;
   const int64_t* mask;
-  const int* bad;
-  int H, stage_all, box;                   // box: cache rows one TMA load takes (page-contiguous)
+  const uint8_t* kv;
+  int H, how;                              // how whole tiles come: FEED, PAGED or STAGED
   float scale_log2;
   const float* sink;
   float* part_o;
@@ -62,83 +65,78 @@ CB_DEVICE uint32_t pack2(float a, float b, bool f16) {
   }
   return pack_bf16x2(a, b);
 }
+CB_DEVICE void store32(void* p, const uint32_t* v) {      // one 32-byte sector (p 32-byte aligned)
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]),
+               "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+               : "memory");
+}
 CB_DEVICE void softmax_sync() { asm volatile("bar.sync 1, %0;" ::"n"(SM_WARPS * 32) : "memory"); }
 
 // ---------------------------------------------------------------------------------------------------------------
-// Rows [tile * 128, ...) of a request -> block of the staging buffer, zeros past its last node.  fp8 rows are expanded
-// to fp16 (exact).  A tree row with a NaN or an infinity is staged as zeros and marked in bad[]: nodes of other
-// branches multiply it by a weight of zero, nodes that see it are made NaN by the attention kernel.  One warp per row.
+// Feeding: a warp brings eight rows into swizzled chunks.  Row r of the CTA's 64, 16-byte piece c of atom a goes to
+// chunk a, byte r * 128 + ((c ^ (r & 7)) << 4).
 // ---------------------------------------------------------------------------------------------------------------
-CB_DEVICE bool nonfinite16(uint32_t v, uint32_t expo) {      // either half has all exponent bits set
-  return (v & expo) == expo || ((v >> 16) & expo) == expo;
+template <bool F8>
+CB_DEVICE bool odd16(const uint4& v) {       // a NaN or an infinity among eight fp16 (F8) / bf16 values
+  constexpr uint32_t e = F8 ? 0x7C00u : 0x7F80u;
+  auto bad = [](uint32_t w) { return (w & e) == e || ((w >> 16) & e) == e; };
+  return bad(v.x) | bad(v.y) | bad(v.z) | bad(v.w);
+}
+// 16 e4m3 values and their atom's UE8M0 scale -> 16 fp16 (exact while the products fit fp16)
+CB_DEVICE void expand16(const uint4& v, uint32_t scale, uint4& a, uint4& b) {
+  const __half2 sc = __float2half2_rn(ue8m0_to_float(scale));
+  uint32_t h[8];
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    uint32_t e;
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(e) : "h"(uint16_t(w[k >> 1] >> (16 * (k & 1)))));
+    const __half2 r = __hmul2(*reinterpret_cast<__half2*>(&e), sc);
+    h[k] = *reinterpret_cast<const uint32_t*>(&r);
+  }
+  a = make_uint4(h[0], h[1], h[2], h[3]);
+  b = make_uint4(h[4], h[5], h[6], h[7]);
+}
+CB_DEVICE void put(uint8_t* chunk, int row, int c, const uint4& v) {
+  *reinterpret_cast<uint4*>(chunk + row * 128 + ((c ^ (row & 7)) << 4)) = v;
 }
 
+// Whole key tiles -> dense fp16 / bf16 rows.  A CTA brings 32 rows, a warp four.
 template <bool F8>
 __global__ void __launch_bounds__(256) tree_stage_kernel(const uint8_t* __restrict__ kv, TreeLayout lay,
                                                          const int2* __restrict__ blocks, int D,
-                                                         uint16_t* __restrict__ staged, int* __restrict__ bad) {
+                                                         uint16_t* __restrict__ staged) {
   pdl_entry();
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31, r0 = (blockIdx.x & 3) * 32 + (threadIdx.x >> 5) * 4;
   const int2 blk = blocks[blockIdx.x >> 2];
-  const int b = blk.x, c = lay.ctx[b], n = lay.cu[b + 1] - lay.cu[b];
+  const int pos = blk.y * KT + r0 + (lane & 3);
+  const int mine = lay.table[size_t(blk.x) * lay.P + pos / lay.page] * lay.page + pos % lay.page;
   const int row_bytes = F8 ? (D == 576 ? 656 : 528) : D * 2;
-  uint32_t v[4][9];
-  int pos[4];
+  uint4 v[4], w[4];
+  uint32_t pe[4], sc[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const int r = (blockIdx.x & 3) * 32 + i * 8 + warp;
-    const int p = pos[i] = blk.y * KT + r;
-#pragma unroll
-    for (int k = 0; k < 9; ++k) v[i][k] = 0;
-    if (p >= c + n) continue;
-    const int slot = lay.table[size_t(b) * lay.P + p / lay.page] * lay.page + p % lay.page;
-    const uint8_t* src = kv + size_t(slot) * row_bytes;
+    const uint8_t* src = kv + int64_t(__shfl_sync(~0u, mine, i)) * row_bytes;
     if constexpr (F8) {
-      const uint4 x = *reinterpret_cast<const uint4*>(src + lane * 16 + (lane >= 16 ? 16 : 0));
-      v[i][0] = x.x; v[i][1] = x.y; v[i][2] = x.z; v[i][3] = x.w;
-      v[i][4] = src[256 + (lane >> 2)];
-      if (D == 576) v[i][8] = reinterpret_cast<const uint32_t*>(src + 528)[lane];
+      v[i] = reinterpret_cast<const uint4*>(src)[lane + (lane >= 16 ? 1 : 0)];
+      sc[i] = src[256 + (lane >> 2)];
     } else {
-      const uint4 x = *reinterpret_cast<const uint4*>(src + lane * 32), y = *reinterpret_cast<const uint4*>(src + lane * 32 + 16);
-      v[i][0] = x.x; v[i][1] = x.y; v[i][2] = x.z; v[i][3] = x.w;
-      v[i][4] = y.x; v[i][5] = y.y; v[i][6] = y.z; v[i][7] = y.w;
-      if (D == 576) v[i][8] = reinterpret_cast<const uint32_t*>(src + 1024)[lane];
+      v[i] = reinterpret_cast<const uint4*>(src)[2 * lane];
+      w[i] = reinterpret_cast<const uint4*>(src)[2 * lane + 1];
     }
+    pe[i] = D == 576 ? reinterpret_cast<const uint32_t*>(src + (F8 ? 528 : 1024))[lane] : 0;
   }
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    uint32_t* w = v[i];
     if constexpr (F8) {
-      if (pos[i] < c + n) {
-        const __half2 sc = __float2half2_rn(ue8m0_to_float(w[4]));
-        uint32_t h[8];
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          uint32_t e;
-          asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(e) : "h"(uint16_t(w[k >> 1] >> (16 * (k & 1)))));
-          const __half2 r = __hmul2(*reinterpret_cast<__half2*>(&e), sc);
-          h[k] = *reinterpret_cast<const uint32_t*>(&r);
-        }
-#pragma unroll
-        for (int k = 0; k < 8; ++k) w[k] = h[k];
-      }
+      uint4 a;
+      expand16(v[i], sc[i], a, w[i]);
+      v[i] = a;
     }
-    if (pos[i] >= c && pos[i] < c + n) {
-      const uint32_t expo = F8 ? 0x7C00u : 0x7F80u;
-      bool odd = false;
-#pragma unroll
-      for (int k = 0; k < 9; ++k) odd |= nonfinite16(w[k], expo);
-      odd = __any_sync(~0u, odd);
-      if (odd)
-#pragma unroll
-        for (int k = 0; k < 9; ++k) w[k] = 0;
-      if (lane == 0) bad[lay.cu[b] + pos[i] - c] = odd;
-    }
-    const int r = (blockIdx.x & 3) * 32 + i * 8 + warp;
-    uint16_t* dst = staged + (size_t(blockIdx.x >> 2) * KT + r) * D;
-    *reinterpret_cast<uint4*>(dst + lane * 16) = make_uint4(w[0], w[1], w[2], w[3]);
-    *reinterpret_cast<uint4*>(dst + lane * 16 + 8) = make_uint4(w[4], w[5], w[6], w[7]);
-    if (D == 576) reinterpret_cast<uint32_t*>(dst + 512)[lane] = w[8];
+    uint16_t* dst = staged + (size_t(blockIdx.x >> 2) * KT + r0 + i) * D;
+    reinterpret_cast<uint4*>(dst)[2 * lane] = v[i];
+    reinterpret_cast<uint4*>(dst)[2 * lane + 1] = w[i];
+    if (D == 576) reinterpret_cast<uint32_t*>(dst + 512)[lane] = pe[i];
   }
 }
 
@@ -149,15 +147,17 @@ __global__ void __launch_bounds__(256) tree_stage_kernel(const uint8_t* __restri
 // CTA 0, 0..3 in CTA 1), so that both CTAs find keys 0-63 in slots 0-3 and keys 64-127 in slots 4-7, as one
 // descriptor has to serve both.  P goes to shared memory (K-major): keys 0-63 over the RoPE chunk (slot 8), keys
 // 64-127 into one extra chunk.
-//   producer (each CTA)  K(0) K(1) V(0) V(1) | K(2) K(3) V(2) V(3) | ...
+//   producer, feed (each CTA)  K(0) K(1) V(0) V(1) | K(2) K(3) V(2) V(3) | ...
 //   MMA (CTA 0)          QK(0) QK(1) PV(0) PV(1) | QK(2) QK(3) PV(2) PV(3) | ...
 //   softmax (each CTA)   thread = (row, 32 of the 128 keys); the four threads of a row exchange their maxima
 // ---------------------------------------------------------------------------------------------------------------
+// A fed row with a NaN or an infinity in a tile that holds tree rows: Q·K^T sees it (its scores are NaN, and so is every
+// node that sees it), but the values P·V multiplies by a weight of zero for the other branches' nodes are made zero.
+//
 // The tensor maps see a row as 64-dim atoms: (64 dims, rows, atoms), so one TMA load fills several chunks.
 struct Maps {
   CUtensorMap q;            // box 64 x 64 rows x all atoms
-  CUtensorMap kv4, kv1;     // cache rows: box 64 x Params::box rows x 4 atoms / 1 atom (the RoPE key)
-  CUtensorMap st4, st1;     // staged rows: 64 rows
+  CUtensorMap kv4, kv1;     // cache rows or staged rows: box 64 x 64 rows x 4 atoms / 1 atom (the RoPE key)
 };
 
 template <int NA, bool F16>
@@ -193,19 +193,22 @@ __global__ void __launch_bounds__(THREADS, 1) tree_mla_kernel(const __grid_const
     mbar_init(q_full, 1);
     mbar_init(o_free, 2 * SM_WARPS);
     for (int i = 0; i < NST; ++i) {
-      mbar_init(&kfull[i], 1); mbar_init(&vfull[i], 1); mbar_init(&sfull[i], 1);
+      // the producer of CTA 0 and the feed warps of both CTAs arrive for every tile
+      mbar_init(&kfull[i], 1 + 2 * FEED_WARPS); mbar_init(&vfull[i], 1 + 2 * FEED_WARPS); mbar_init(&sfull[i], 1);
       mbar_init(&p0full[i], 2 * SM_WARPS); mbar_init(&p1full[i], SM_WARPS); mbar_init(&pv0[i], 1); mbar_init(&pv1[i], 1);
     }
     *abort_flag = 0;
     fence_barrier_init();
   }
   if (warp == 2) { tmem_alloc_pair(tmem_slot, 512); tmem_relinquish_pair(); }
+  const int i0 = p.work.first[cluster], i1 = p.work.first[cluster + 1];   // made by the host: no kernel writes them
   tc_fence_before();
   cluster_sync();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  pdl_entry();
-  const int i0 = p.work.first[cluster], i1 = p.work.first[cluster + 1];
+  // Items and page table are made by the host: the roles look up their first rows before they wait for the kernel that
+  // wrote the queries and the cache.
+  pdl_launch_dependents();
   auto fail = [&](int code) { if (p.status) atomicCAS(p.status, 0, code); *abort_flag = 1; };
   auto wait = [&](uint64_t* bar, uint32_t phase, int code) -> bool {
     if (mbar_wait(bar, phase)) return true;
@@ -213,75 +216,68 @@ __global__ void __launch_bounds__(THREADS, 1) tree_mla_kernel(const __grid_const
     return false;
   };
 
+  // whether a key tile comes by TMA
+  auto by_tma = [&](const TreeItem& it, int tile) { return p.how != FEED && (tile + 1) * KT <= it.ctx; };
+
   if (warp == 0) {
-    // ---------------- producer ----------------
+    // ---------------- producer: Q and the key tiles that TMA can take ----------------
     if (lane == 0) {
       tma_prefetch_desc(&tm.q); tma_prefetch_desc(&tm.kv4); tma_prefetch_desc(&tm.kv1);
-      tma_prefetch_desc(&tm.st4); tma_prefetch_desc(&tm.st1);
       const uint32_t lead_q = mapa_shared(smem_u32(q_full), 0);
       int g = 0;                                        // tiles so far: stage g % 2, phase (g / 2) & 1
       bool ok = true;
       for (int i = i0; ok && i < i1; ++i) {
         const TreeItem it = p.work.items[i];
-        const int ctx = p.lay.ctx[it.b];
-        const int staged_from = p.stage_all ? 0 : ctx / KT;
         const int* table = p.lay.table + size_t(it.b) * p.lay.P;
-        // n atoms from atom a of 64 keys (half `half` of a tile) -> chunks.  The first rows of a tile's boxes are looked
-        // up ahead of the waits: a page-table read per load would cost more than the load's issue.
-        auto row_of = [&](int tile, int half, int r) -> int {
-          if (tile >= staged_from) return (p.work.stage_at[it.b] + tile - staged_from) * KT + half * 64 + r;
-          const int pos = tile * KT + half * 64 + r;
+        const int staged = p.how == STAGED ? p.work.stage_at[it.b] * KT : 0;
+        auto row_of = [&](int tile, int half) -> int {  // row of a half tile's first key
+          if (p.how == STAGED) return staged + tile * KT + half * 64;
+          const int pos = tile * KT + half * 64;
           return table[pos / p.lay.page] * p.lay.page + pos % p.lay.page;
         };
-        auto load = [&](uint8_t* dst, uint32_t bar, int tile, int half, int row0, int a, bool four) {
-          if (tile >= staged_from) {
-            tma_load_3d_pair(dst, four ? &tm.st4 : &tm.st1, bar, 0, row0, a);
-          } else if (p.box == 64) {
-            tma_load_3d_pair(dst, four ? &tm.kv4 : &tm.kv1, bar, 0, row0, a);
-          } else {              // a box shorter than a chunk: one atom at a time
-            for (int r = 0; r < 64; r += p.box) {
-              const int row = r ? row_of(tile, half, r) : row0;
-              for (int k = 0; k < (four ? 4 : 1); ++k)
-                tma_load_3d_pair(dst + k * CH + r * 128, &tm.kv1, bar, 0, row, a + k);
-            }
-          }
-        };
-        // L2 prefetch of the CTA's half of a tile two tiles before its load: the ring holds two tiles, too few to cover
-        // the latency of HBM
-        auto prefetch = [&](int tile) {
-          if (tile >= staged_from || p.box != 64) return;
-          const int row = row_of(tile, rank, 0);
-          tma_prefetch_l2_3d(&tm.kv4, 0, row, 0);
-          tma_prefetch_l2_3d(&tm.kv4, 0, row, 4);
-          if (NA == 9) tma_prefetch_l2_3d(&tm.kv1, 0, row, 8);
-        };
+        if (i == i0) pdl_wait();
         // Q: the previous item's last Q·K^T is done (its V loads waited for it)
         if (rank == 0) mbar_arrive_expect_tx(q_full, 2 * NA * CH);
-        const int q_row = p.lay.cu[it.b] * p.H + it.row * 128 + rank * 64;
-        tma_load_3d_pair(sQ, &tm.q, lead_q, 0, q_row, 0);
+        tma_load_3d_pair(sQ, &tm.q, lead_q, 0, it.c0 * p.H + it.row * 128 + rank * 64, 0);
         for (int j = 0; ok && j < it.n_tiles; j += 2) {
           const int m = min(2, it.n_tiles - j);
           for (int u = 0; ok && u < m; ++u) {
-            const int s = (g + u) & 1, ph = ((g + u) >> 1) & 1;
+            const int s = (g + u) & 1, ph = ((g + u) >> 1) & 1, tile = it.tile + j + u;
+            const bool tma = by_tma(it, tile);
             uint8_t* st = sK + s * STAGE;
             const uint32_t bar = mapa_shared(smem_u32(&kfull[s]), 0);
-            const int tile = it.tile + j + u, row0 = row_of(tile, rank, 0);
-            if (rank == 0) mbar_arrive_expect_tx(&kfull[s], 2 * NA * CH);
+            const int row = tma ? row_of(tile, rank) : 0;       // looked up ahead of the waits
             if (!(ok = wait(&pv0[s], ph ^ 1, kErrTimeoutEmpty))) break;
-            load(st, bar, tile, rank, row0, 0, true);
-            if (NA == 9) load(st + 8 * CH, bar, tile, rank, row0, 8, false);
+            if (rank == 0) {
+              if (tma) mbar_arrive_expect_tx(&kfull[s], 2 * NA * CH);
+              else mbar_arrive(&kfull[s]);
+            }
+            if (tma) {
+              tma_load_3d_pair(st, &tm.kv4, bar, 0, row, 0);
+              if (NA == 9) tma_load_3d_pair(st + 8 * CH, &tm.kv1, bar, 0, row, 8);
+            }
             if (!(ok = wait(&pv1[s], ph ^ 1, kErrTimeoutEmpty))) break;
-            load(st + 4 * CH, bar, tile, rank, row0, 4, true);
-            if (j + u + 2 < it.n_tiles) prefetch(tile + 2);
+            if (tma) tma_load_3d_pair(st + 4 * CH, &tm.kv4, bar, 0, row, 4);
+            // L2 prefetch of the CTA's half two tiles on: the ring holds two tiles, too few to cover the latency of HBM
+            if (j + u + 2 < it.n_tiles && by_tma(it, tile + 2)) {
+              const int r2 = row_of(tile + 2, rank);
+              tma_prefetch_l2_3d(&tm.kv4, 0, r2, 0);
+              tma_prefetch_l2_3d(&tm.kv4, 0, r2, 4);
+              if (NA == 9) tma_prefetch_l2_3d(&tm.kv1, 0, r2, 8);
+            }
           }
           for (int u = 0; ok && u < m; ++u) {
-            const int s = (g + u) & 1, ph = ((g + u) >> 1) & 1;
-            uint8_t* st = sK + s * STAGE;
-            const uint32_t bar = mapa_shared(smem_u32(&vfull[s]), 0);
-            const int tile = it.tile + j + u, row0 = row_of(tile, rank ^ 1, 0);
-            if (rank == 0) mbar_arrive_expect_tx(&vfull[s], 2 * 4 * CH);
+            const int s = (g + u) & 1, ph = ((g + u) >> 1) & 1, tile = it.tile + j + u;
+            const bool tma = by_tma(it, tile);
+            const int row = tma ? row_of(tile, rank ^ 1) : 0;
             if (!(ok = wait(&sfull[s], ph, kErrTimeoutFull))) break;
-            load(st + (rank ? 0 : 4) * CH, bar, tile, rank ^ 1, row0, 4 * rank, true);
+            if (rank == 0) {
+              if (tma) mbar_arrive_expect_tx(&vfull[s], 2 * 4 * CH);
+              else mbar_arrive(&vfull[s]);
+            }
+            if (tma)
+              tma_load_3d_pair(sK + s * STAGE + (rank ? 0 : 4) * CH, &tm.kv4, mapa_shared(smem_u32(&vfull[s]), 0), 0,
+                               row, 4 * rank);
           }
           g += m;
         }
@@ -290,6 +286,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_mla_kernel(const __grid_const
     }
   } else if (warp == 1) {
     // ---------------- MMA (the leader issues for both CTAs) ----------------
+    pdl_wait();
     if (rank == 0 && elect_one()) {
       const uint32_t id_qk = F16 ? idesc_f16(128, KT) : idesc_bf16(128, KT);
       const uint32_t id_pv = (F16 ? idesc_f16(128, 256) : idesc_bf16(128, 256)) | (1u << 16);   // V is MN-major
@@ -342,17 +339,191 @@ __global__ void __launch_bounds__(THREADS, 1) tree_mla_kernel(const __grid_const
         }
       }
     }
-  } else if (warp >= 4) {
+  } else if (warp < 2 + FEED_WARPS) {
+    // ---------------- feed: rows r0 .. r0 + 7 of the CTA's 64 keys (K) and of the peer's (V) ----------------
+    // A tile's loads are issued before the wait for its slots; the slots' cache rows were looked up a pair of tiles
+    // earlier (a dependent page-table read per tile would cost as much as the conversion).
+    constexpr bool F8 = F16;
+    constexpr int RB = F8 ? (NA == 9 ? 656 : 528) : NA * 128;
+    const int r0 = (int(warp) - 2) * 8;
+    const uint4 zero = make_uint4(0, 0, 0, 0);
+    int g = 0;
+    bool ok = true;
+    for (int i = i0; ok && i < i1; ++i) {
+      const TreeItem it = p.work.items[i];
+      const int* table = p.lay.table + size_t(it.b) * p.lay.P;
+      const int end = it.ctx + it.n, nt = it.n_tiles;
+      // lane r < 8: cache row of row r0 + r of a half tile (rows past the end: the last row's)
+      auto row_of = [&](int j, int half) -> int {
+        if (j >= nt || by_tma(it, it.tile + j)) return 0;
+        const int pos = min((it.tile + j) * KT + half * 64 + r0 + int(lane & 7), end - 1);
+        return table[pos / p.lay.page] * p.lay.page + pos % p.lay.page;
+      };
+      auto at = [&](int rows, int r) { return p.kv + int64_t(__shfl_sync(~0u, rows, r)) * RB; };
+      uint32_t odd = 0;                                 // this warp's rows with a NaN or an infinity, 8 bits per stage
+      int k0 = row_of(0, rank), k1 = row_of(1, rank), v0 = row_of(0, rank ^ 1), v1 = row_of(1, rank ^ 1);
+      if (i == i0) pdl_wait();
+      for (int j = 0; ok && j < nt; j += 2) {
+        const int m = min(2, nt - j);
+        const int nk0 = row_of(j + 2, rank), nk1 = row_of(j + 3, rank);
+        const int nv0 = row_of(j + 2, rank ^ 1), nv1 = row_of(j + 3, rank ^ 1);
+        for (int u = 0; ok && u < m; ++u) {
+          const int s = (g + u) & 1, ph = ((g + u) >> 1) & 1, tile = it.tile + j + u;
+          uint8_t* st = sK + s * STAGE;
+          const bool fed = !by_tma(it, tile), tail = (tile + 1) * KT > it.ctx;
+          if (fed) {
+            const int mine = u ? k1 : k0;
+            const int rows = end - (tile * KT + rank * 64 + r0);        // rows of this warp that exist
+            odd &= ~(0xFFu << (8 * s));
+            uint4 pe[2];                                // RoPE pieces: lane = (row of four, piece)
+            auto load_pe = [&]() {
+#pragma unroll
+              for (int k = 0; k < 2; ++k)
+                if (NA == 9) pe[k] = reinterpret_cast<const uint4*>(at(mine, 4 * k + (lane >> 3)))[(F8 ? 33 : 64) + (lane & 7)];
+            };
+            auto store_pe = [&]() {
+#pragma unroll
+              for (int k = 0; k < 2; ++k) {
+                if (NA != 9) break;
+                if (tail && 4 * k + int(lane >> 3) >= rows) pe[k] = zero;
+                put(st + 8 * CH, r0 + 4 * k + (lane >> 3), lane & 7, pe[k]);
+                if (tail) {
+                  const uint32_t bad = __ballot_sync(~0u, odd16<F8>(pe[k]));
+#pragma unroll
+                  for (int r = 0; r < 4; ++r)
+                    if ((bad >> (8 * r)) & 0xFF) odd |= 1u << (8 * s + 4 * k + r);
+                }
+              }
+            };
+            if constexpr (F8) {
+              uint4 v[8];
+              uint32_t sc[8];
+#pragma unroll
+              for (int r = 0; r < 8; ++r) {
+                const uint8_t* src = at(mine, r);
+                v[r] = reinterpret_cast<const uint4*>(src)[lane + (lane >= 16 ? 1 : 0)];
+                sc[r] = src[256 + (lane >> 2)];
+              }
+              load_pe();
+              ok = wait(&pv0[s], ph ^ 1, kErrTimeoutEmpty) && wait(&pv1[s], ph ^ 1, kErrTimeoutEmpty);
+#pragma unroll
+              for (int r = 0; r < 8; ++r) {
+                uint4 a, b;
+                if (tail && r >= rows) v[r] = zero;
+                expand16(v[r], sc[r], a, b);
+                // lanes of odd atoms store their second piece first: all eight 16-byte columns in each store
+                uint8_t* ch = st + (lane >> 2) * CH;
+                const int c = 2 * (lane & 3), sw = (lane >> 2) & 1;
+                put(ch, r0 + r, c + sw, sw ? b : a);
+                put(ch, r0 + r, c + (sw ^ 1), sw ? a : b);
+                if (tail && __any_sync(~0u, odd16<F8>(a) || odd16<F8>(b))) odd |= 1u << (8 * s + r);
+              }
+              store_pe();
+            } else {
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {             // four rows at a time
+                uint4 v[8];
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+#pragma unroll
+                  for (int k = 0; k < 2; ++k) v[2 * r + k] = reinterpret_cast<const uint4*>(at(mine, 4 * h + r))[k * 32 + lane];
+                if (h == 0) {
+                  load_pe();
+                  ok = wait(&pv0[s], ph ^ 1, kErrTimeoutEmpty) && wait(&pv1[s], ph ^ 1, kErrTimeoutEmpty);
+                }
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                  if (tail && 4 * h + r >= rows) v[2 * r] = v[2 * r + 1] = zero;
+#pragma unroll
+                  for (int k = 0; k < 2; ++k)
+                    put(st + (k * 4 + (lane >> 3)) * CH, r0 + 4 * h + r, lane & 7, v[2 * r + k]);
+                  if (tail && __any_sync(~0u, odd16<F8>(v[2 * r]) || odd16<F8>(v[2 * r + 1])))
+                    odd |= 1u << (8 * s + 4 * h + r);
+                }
+              }
+              store_pe();
+            }
+            fence_proxy_async();
+          } else {
+            ok = wait(&pv1[s], ph ^ 1, kErrTimeoutEmpty);
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive_cluster(mapa_shared(smem_u32(&kfull[s]), 0));
+          if (fed && j + u + 2 < nt && !by_tma(it, tile + 2)) {         // L2 prefetch two tiles on
+            const uint8_t* row = p.kv + int64_t(__shfl_sync(~0u, u ? nk1 : nk0, lane >> 2)) * RB;
+#pragma unroll
+            for (int o = 0; o < RB; o += 512)
+              if (o + int(lane & 3) * 128 < RB) asm volatile("prefetch.global.L2 [%0];" ::"l"(row + o + (lane & 3) * 128));
+          }
+        }
+        for (int u = 0; ok && u < m; ++u) {
+          const int s = (g + u) & 1, ph = ((g + u) >> 1) & 1, tile = it.tile + j + u;
+          uint8_t* st = sK + s * STAGE;
+          if (!by_tma(it, tile)) {
+            const bool tail = (tile + 1) * KT > it.ctx;
+            const int mine = u ? v1 : v0;
+            const int rows = end - (tile * KT + (rank ^ 1) * 64 + r0);
+            uint8_t* dst = st + (rank ? 0 : 4) * CH;
+            if constexpr (F8) {
+              uint4 v[4];                               // two rows per load: 16 lanes x 16 values
+              uint32_t sc[4];
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                const uint8_t* src = at(mine, 2 * k + (lane >> 4));
+                v[k] = reinterpret_cast<const uint4*>(src)[17 * rank + (lane & 15)];
+                sc[k] = src[256 + 4 * rank + ((lane & 15) >> 2)];
+              }
+              ok = wait(&sfull[s], ph, kErrTimeoutFull);
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                uint4 a, b;
+                if (tail && 2 * k + int(lane >> 4) >= rows) v[k] = zero;
+                expand16(v[k], sc[k], a, b);
+                if (tail && odd16<F8>(a)) a = zero;
+                if (tail && odd16<F8>(b)) b = zero;
+                const int row = r0 + 2 * k + (lane >> 4), c = 2 * (lane & 3), sw = (lane >> 2) & 1;
+                uint8_t* ch = dst + ((lane & 15) >> 2) * CH;
+                put(ch, row, c + sw, sw ? b : a);
+                put(ch, row, c + (sw ^ 1), sw ? a : b);
+              }
+            } else {
+              uint4 v[8];
+#pragma unroll
+              for (int r = 0; r < 8; ++r) v[r] = reinterpret_cast<const uint4*>(at(mine, r))[32 * rank + lane];
+              ok = wait(&sfull[s], ph, kErrTimeoutFull);
+#pragma unroll
+              for (int r = 0; r < 8; ++r) {
+                if (tail && (r >= rows || odd16<F8>(v[r]))) v[r] = zero;
+                put(dst + (lane >> 3) * CH, r0 + r, lane & 7, v[r]);
+              }
+            }
+            // this CTA's own keys: rows that were marked lose their values
+            for (uint32_t left = (odd >> (8 * s)) & 0xFF; left; left &= left - 1)
+              put(st + (4 * rank + (lane >> 3)) * CH, r0 + __ffs(left) - 1, lane & 7, zero);
+            fence_proxy_async();
+          } else {
+            ok = wait(&sfull[s], ph, kErrTimeoutFull);
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive_cluster(mapa_shared(smem_u32(&vfull[s]), 0));
+        }
+        g += m;
+        k0 = nk0; k1 = nk1; v0 = nv0; v1 = nv1;
+      }
+      if (*abort_flag) ok = false;
+    }
+  } else {
     // ---------------- softmax, rescale, epilogue: lanes 0-63 / 64-127 hold the first / second 64 keys of the rows;
     // two warps share 32 lanes and take 32 score columns (and 128 of the 256 columns of O) each -------
-    const int q = warp & 3, half = q >> 1, row = (q & 1) * 32 + int(lane), part = (int(warp) - 4) >> 2;
+    const int q = warp & 3, half = q >> 1, row = (q & 1) * 32 + int(lane), part = (int(warp) - 2 - FEED_WARPS) >> 2;
     const int me = part * 128 + q * 32 + int(lane);
     const uint32_t t_lane = tmem + (uint32_t(q * 32) << 16);
+    pdl_wait();
     int g = 0;
     bool ok = true;                       // after a failed wait the loop runs on without waiting: the block-level
     for (int i = i0; i < i1; ++i) {       // barriers below need all the warps
       const TreeItem it = p.work.items[i];
-      const int ctx = p.lay.ctx[it.b], c0 = p.lay.cu[it.b], n = p.lay.cu[it.b + 1] - c0;
+      const int ctx = it.ctx, c0 = it.c0, n = it.n;
       const int r = it.row * 128 + rank * 64 + row;
       const bool live = r < n * p.H;
       const int node = live ? r / p.H : 0, head = r - node * p.H;
@@ -392,13 +563,13 @@ __global__ void __launch_bounds__(THREADS, 1) tree_mla_kernel(const __grid_const
           ok = ok && wait(&pv1[s ^ 1], ((g - 1) >> 1) & 1, kErrTimeoutTmem);
           tc_fence_after();
 #pragma unroll 1
-          for (int c = part * 128; c < part * 128 + 128; c += 32) {
-            uint32_t o[32];
-            tmem_ld_32x32b_x32(t_lane + TM_O + c, o);
+          for (int c = part * 128; c < part * 128 + 128; c += 16) {
+            uint32_t o[16];
+            tmem_ld_32x32b_x16(t_lane + TM_O + c, o);
             tmem_ld_wait();
 #pragma unroll
-            for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * keep);
-            tmem_st_32x32b_x32(t_lane + TM_O + c, o);
+            for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * keep);
+            tmem_st_32x32b_x16(t_lane + TM_O + c, o);
           }
           tmem_st_wait();
           l *= keep;
@@ -434,11 +605,6 @@ __global__ void __launch_bounds__(THREADS, 1) tree_mla_kernel(const __grid_const
       const int sl = (g - 1) & 1;
       ok = ok && wait(&pv1[sl], ((g - 1) >> 1) & 1, kErrTimeoutTmem);
       tc_fence_after();
-      if ((it.tile + it.n_tiles) * KT > ctx) {            // nodes that see a marked row become NaN
-        const int b0 = int(lane) < n ? p.bad[c0 + lane] : 0, b1 = int(lane) + 32 < n ? p.bad[c0 + 32 + lane] : 0;
-        const uint64_t bad = uint64_t(__ballot_sync(~0u, b0)) | uint64_t(__ballot_sync(~0u, b1)) << 32;
-        if (mask & bad) l = __int_as_float(0x7fffffff);
-      }
       // sums: the maxima buffer of the tile before last is free, and the next item's first tile takes it only after
       // every warp passed the second barrier
       float* xs = xm + (g & 1) * 256;
@@ -464,16 +630,13 @@ __global__ void __launch_bounds__(THREADS, 1) tree_mla_kernel(const __grid_const
         tmem_ld_wait();
         if (it.part >= 0) {
 #pragma unroll
-          for (int k = 0; k < 8; ++k)
-            reinterpret_cast<uint4*>(po + c)[k] = make_uint4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]);
+          for (int k = 0; k < 32; k += 8) store32(po + c + k, v + k);
         } else if (live) {
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
-            reinterpret_cast<uint4*>(o + c)[k] =
-                make_uint4(pack_bf16x2(__uint_as_float(v[8 * k]) * inv, __uint_as_float(v[8 * k + 1]) * inv),
-                           pack_bf16x2(__uint_as_float(v[8 * k + 2]) * inv, __uint_as_float(v[8 * k + 3]) * inv),
-                           pack_bf16x2(__uint_as_float(v[8 * k + 4]) * inv, __uint_as_float(v[8 * k + 5]) * inv),
-                           pack_bf16x2(__uint_as_float(v[8 * k + 6]) * inv, __uint_as_float(v[8 * k + 7]) * inv));
+          for (int k = 0; k < 16; ++k)
+            v[k] = pack_bf16x2(__uint_as_float(v[2 * k]) * inv, __uint_as_float(v[2 * k + 1]) * inv);
+          store32(o + c, v);
+          store32(o + c + 16, v + 8);
         }
       }
       tc_fence_before();
@@ -490,36 +653,46 @@ __global__ void __launch_bounds__(THREADS, 1) tree_mla_kernel(const __grid_const
 }
 
 // out = sum_s 2^(m_s - M) O_s / (sum_s 2^(m_s - M) l_s + sink): one CTA per row of a split row tile, four of the 512
-// dims per thread, eight partial rows in flight.
-__global__ void __launch_bounds__(128) tree_merge_kernel(TreeLayout lay, const TreeMerge* __restrict__ merges, int H,
+// dims per thread; eight partial rows are in flight, with a running maximum.
+__global__ void __launch_bounds__(128) tree_merge_kernel(const TreeMerge* __restrict__ merges, int H,
                                                          const float* __restrict__ part_o,
                                                          const float* __restrict__ part_ml,
                                                          const float* __restrict__ sink,
                                                          __nv_bfloat16* __restrict__ out) {
+  const TreeMerge mg = merges[blockIdx.x];              // made by the host
   pdl_entry();
-  const TreeMerge mg = merges[blockIdx.x];
-  const int row = blockIdx.y;
-  const int r = mg.row * 128 + row, n = lay.cu[mg.b + 1] - lay.cu[mg.b];
-  if (r >= n * H) return;
+  const int row = blockIdx.y, r = mg.row * 128 + row;
+  if (r >= mg.rows) return;
   const float2* ml = reinterpret_cast<const float2*>(part_ml) + size_t(mg.part) * 128 + row;
-  const float sk = sink ? sink[r % H] * 1.4426950408889634f : -INFINITY;
-  float M = sk;
-#pragma unroll 8
-  for (int s = 0; s < mg.n; ++s) M = fmaxf(M, ml[s * 128].x);
-  if (M == -INFINITY) M = 0.f;
-  float L = exp2f(sk - M);
-  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
   const float4* po = reinterpret_cast<const float4*>(part_o) + (size_t(mg.part) * 128 + row) * 128 + threadIdx.x;
-#pragma unroll 8
-  for (int s = 0; s < mg.n; ++s) {
-    const float2 v = ml[s * 128];
-    const float4 o = po[size_t(s) * 128 * 128];
-    const float w = exp2f(v.x - M);
-    L += w * v.y;
-    acc.x += w * o.x; acc.y += w * o.y; acc.z += w * o.z; acc.w += w * o.w;
+  float M = sink ? sink[r % H] * 1.4426950408889634f : -INFINITY;
+  float L = sink ? 1.f : 0.f;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int s0 = 0; s0 < mg.n; s0 += 8) {
+    float2 v[8];
+    float4 o[8];
+#pragma unroll
+    for (int s = 0; s < 8; ++s) {
+      const bool in = s0 + s < mg.n;
+      v[s] = in ? ml[(s0 + s) * 128] : make_float2(-INFINITY, 0.f);
+      o[s] = in ? po[size_t(s0 + s) * 128 * 128] : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    float top = M;
+#pragma unroll
+    for (int s = 0; s < 8; ++s) top = fmaxf(top, v[s].x);
+    const float ref = top == -INFINITY ? 0.f : top, keep = exp2f(M - ref);
+    acc.x *= keep; acc.y *= keep; acc.z *= keep; acc.w *= keep;
+    L *= keep;
+    M = top;
+#pragma unroll
+    for (int s = 0; s < 8; ++s) {
+      const float w = exp2f(v[s].x - ref);
+      L += w * v[s].y;
+      acc.x += w * o[s].x; acc.y += w * o[s].y; acc.z += w * o[s].z; acc.w += w * o[s].w;
+    }
   }
   const float inv = L == 0.f ? 0.f : 1.f / L;
-  reinterpret_cast<uint2*>(out + (size_t(lay.cu[mg.b]) * H + r) * 512)[threadIdx.x] =
+  reinterpret_cast<uint2*>(out + (size_t(mg.c0) * H + r) * 512)[threadIdx.x] =
       make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
 }
 
@@ -574,32 +747,30 @@ int tree_mla_clusters() {
   return cudaOccupancyMaxActiveClusters(&n, f, &cfg) == cudaSuccess ? n : 0;
 }
 
-cudaError_t tree_mla(const void* q, int T, int H, int D, bool f8, bool all, const void* kv, int64_t S,
-                     const TreeLayout& lay, const TreeWork& work, const int64_t* mask, float scale, const float* sink,
-                     void* staged, int* bad, float* part_o, float* part_ml, int* status, void* out, cudaStream_t s) {
+cudaError_t tree_mla(const void* q, int T, int H, int D, bool f8, const void* kv, int64_t S, const TreeLayout& lay,
+                     const TreeWork& work, const int64_t* mask, float scale, const float* sink, float* part_o,
+                     float* part_ml, void* staged, int* status, void* out, cudaStream_t s) {
   using namespace tree;
   if (!encode_fn()) return cudaErrorNotSupported;
   if (D != 576 && D != 512) return cudaErrorInvalidValue;
-  int box = 64;
-  while (lay.page % box) box /= 2;
-  if (box < 8 && !all) return cudaErrorInvalidValue;
+  const int how = staged ? STAGED : f8 || lay.page % 64 != 0 ? FEED : PAGED;
+  cudaError_t e;
   Maps m;
-  const int64_t st_rows = int64_t(work.n_stage) * KT;
-  if (!row_map(&m.q, f8, q, int64_t(T) * H, D, 64, D / 64) || !row_map(&m.st4, f8, staged, st_rows, D, 64, 4) ||
-      !row_map(&m.st1, f8, staged, st_rows, D, 64, 1))
+  if (!row_map(&m.q, f8, q, int64_t(T) * H, D, 64, D / 64)) return cudaErrorInvalidValue;
+  m.kv4 = m.kv1 = m.q;
+  const void* rows = staged ? staged : kv;
+  const int64_t n_rows = staged ? int64_t(work.n_stage) * KT : S;
+  if (how != FEED && !(row_map(&m.kv4, f8, rows, n_rows, D, 64, 4) && row_map(&m.kv1, f8, rows, n_rows, D, 64, 1)))
     return cudaErrorInvalidValue;
-  m.kv4 = m.st4;
-  m.kv1 = m.st1;
-  if (!all && !(row_map(&m.kv4, false, kv, S, D, box, 4) && row_map(&m.kv1, false, kv, S, D, box, 1)))
-    return cudaErrorInvalidValue;
-  const auto* kvb = reinterpret_cast<const uint8_t*>(kv);
-  auto* st = reinterpret_cast<uint16_t*>(staged);
-  cudaError_t e = launch_k(f8 ? tree_stage_kernel<true> : tree_stage_kernel<false>, dim3(work.n_stage * 4), 256, 0, s,
-                           kvb, lay, work.stage, D, st, bad);
-  if (e != cudaSuccess) return e;
+  if (staged &&
+      (e = launch_k(f8 ? tree_stage_kernel<true> : tree_stage_kernel<false>, dim3(work.n_stage * 4), 256, 0, s,
+                    reinterpret_cast<const uint8_t*>(kv), lay, work.stage, D, reinterpret_cast<uint16_t*>(staged))) !=
+          cudaSuccess)
+    return e;
   Params p;
-  p.lay = lay; p.work = work; p.mask = mask; p.bad = bad;
-  p.H = H; p.stage_all = all; p.box = box;
+  p.lay = lay; p.work = work; p.mask = mask;
+  p.kv = reinterpret_cast<const uint8_t*>(kv);
+  p.H = H; p.how = how;
   p.scale_log2 = scale * 1.4426950408889634f;
   p.sink = sink; p.part_o = part_o; p.part_ml = part_ml; p.status = status;
   p.out = reinterpret_cast<__nv_bfloat16*>(out);
@@ -609,7 +780,7 @@ cudaError_t tree_mla(const void* q, int T, int H, int D, bool f8, bool all, cons
   cudaLaunchAttribute attr[2];
   const cudaLaunchConfig_t cfg = pair_config(work.clusters, attr, s);
   if ((e = cudaLaunchKernelEx(&cfg, f, m, p)) != cudaSuccess || !work.n_merges) return e;
-  return launch_k(tree_merge_kernel, dim3(work.n_merges, 128), 128, 0, s, lay, work.merges, H, part_o, part_ml, sink,
+  return launch_k(tree_merge_kernel, dim3(work.n_merges, 128), 128, 0, s, work.merges, H, part_o, part_ml, sink,
                   p.out);
 }
 

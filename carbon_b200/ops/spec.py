@@ -86,7 +86,6 @@ class TreePlan:
             req += [b] * k
             par += p
             pos += [c + d for d in depth]
-        self._ws = {}
         self.ctx_list, self.tables_list, self.parents_list = [int(c) for c in ctx], page_tables, parents
         self.cu_list, self.pos_list = cu, pos
         self.max_page = max((pg for tab in page_tables for pg in tab), default=-1)
@@ -95,7 +94,7 @@ class TreePlan:
         for tab in page_tables:
             flat += list(tab)
             flat += [0] * (P - len(tab))
-        # one host buffer, one copy: masks (64 bits) first, the attention's work (64-bit aligned), the 32-bit lists
+        # one host buffer, one copy: the attention's work (16-byte aligned parts), masks (64 bits), the 32-bit lists
         T = self.T
         words = torch.tensor(bits, dtype=torch.int64).view(torch.int32)
         work, self._counts = torch.zeros(0, dtype=torch.int32), []
@@ -103,35 +102,21 @@ class TreePlan:
             work, self._counts = ext().tree_schedule(self.n, [int(c) for c in ctx], self.n_heads,
                                                      _clusters(self.device))
         ints = torch.tensor(cu + list(ctx) + req + par + pos + flat + [0], dtype=torch.int32)
-        host = torch.cat([words, work, ints])
+        host = torch.cat([work, words, ints])
         if self.device.type == "cuda":
             host = host.pin_memory()
         dev = host.to(self.device, non_blocking=True)
-        self.mask = dev[:2 * T].view(torch.int64)
-        self._work = dev[2 * T:2 * T + work.numel()]
+        w = work.numel()                    # a multiple of 4
+        self._work = dev[:w]
+        self.mask = dev[w:w + 2 * T].view(torch.int64)
         self.status = dev[-1:]              # error code of a device-side wait that ran out (0: none)
-        at = 2 * T + work.numel()
+        at = w + 2 * T
         out = []
         for k in (B + 1, B, T, T, T, B * P):
             out.append(dev[at:at + k])
             at += k
         self.cu, self.ctx, self.req, self.parent, self.pos, self.table = out
         self.table = self.table.view(B, P)
-
-    def _workspace(self, f8: bool, D: int):
-        """(whether every row is staged, byte offsets of the workspace's parts, its size) of an attention call.  Rows
-        that TMA cannot take from the cache as they lie are staged in a dense 16-bit buffer: fp8 rows, and pages that
-        are no multiple of 8 rows (a swizzle group); else only each request's last tiles."""
-        got = self._ws.get((f8, D))
-        if got is None:
-            whole = f8 or self.page_size % 8 != 0
-            parts = self._counts[3]
-            off, end = [], 0
-            for k in (self._counts[5 if whole else 4] * 256 * D, 4 * self.T, parts * 128 * 2048, parts * 128 * 8):
-                off.append(end)
-                end += (k + 255) // 256 * 256
-            got = self._ws[(f8, D)] = (whole, off, end)
-        return got
 
     def check(self) -> None:
         """Raise if a kernel of this plan gave up a wait (reads from the device)."""
@@ -200,11 +185,18 @@ def tree_mla(q: torch.Tensor, kv: torch.Tensor, plan: TreePlan, scale: float, d_
             _need("tree_mla: sink", sink, dev, torch.float32)
         out = torch.empty(T, H, 512, dtype=torch.bfloat16, device=q.device)
         if T:
-            whole, off, size = plan._workspace(f8, D)
-            buf = torch.empty(size, dtype=torch.uint8, device=q.device)
-            _launched(ext().tree_mla(qk, kv, plan.cu, plan.ctx, plan.table, plan.mask, plan.page_size, whole,
-                                     plan._work, plan._counts, buf, off, float(scale), sink, plan.status, out),
-                      "tree_mla")
+            parts, tiles, work = plan._counts[3:]
+            # Whole key tiles that TMA cannot take from the cache as they lie (fp8 rows, small pages) are fed by the
+            # kernel's warps (4.0 us a tile and CTA pair), or expanded to dense rows first (2.0 us a tile then, and
+            # 2.8 us of every pair's time per staged tile; a launch): worth it from two row tiles per key tile and a
+            # few tiles per pair on.  32 requests near 4096, 6 nodes of 128 heads: 216 us fed, 152 us staged; one
+            # node: 70 us fed, 96 us staged; 4 requests of 500, 8 nodes: 23.8 us fed, 25.0 us staged.
+            staged = None
+            if (f8 or plan.page_size % 64) and tiles and work >= 2 * tiles and work >= 4 * plan._counts[0]:
+                staged = torch.empty(tiles * 128 * D, dtype=want, device=q.device)
+            buf = torch.empty(parts * 128 * 514, dtype=torch.float32, device=q.device) if parts else None
+            _launched(ext().tree_mla(qk, kv, plan.cu, plan.ctx, plan.table, plan.mask, plan.page_size, plan._work,
+                                     plan._counts, buf, staged, float(scale), sink, plan.status, out), "tree_mla")
         return out
     out = torch.zeros(T, H, d_latent)
     mla = D > d_latent
