@@ -23,66 +23,89 @@ CB_DEVICE float ex2v(float x) {
 // CTA's slot array through distributed shared memory; two arrays alternate, so that one exchange's slots are read
 // before the next but one writes them.  WARP reduces a float4 over the first `w` lanes of a warp (w a power of two).
 struct Exchange {
-  float4 (*slots)[kMaxCluster];     // [2][kMaxCluster]
-  float4* warps;                    // [kThreads / 32]
+  float4 (*slots)[2][kMaxCluster];  // [2][2][kMaxCluster]
+  float4 (*warps)[2];               // [kThreads / 32][2]
   int n, rank, turn;
+  // over(a, b, w): both values reduced over the first w lanes; b only if `two`
   template <typename WARP>
-  CB_DEVICE float4 reduce(float4 v, WARP over) {
+  CB_DEVICE void reduce(float4& a, float4& b, bool two, WARP over) {
     const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
-    v = over(v, 32);
-    if (lane == 0) warps[wid] = v;
+    over(a, b, 32);
+    if (lane == 0) {
+      warps[wid][0] = a;
+      if (two) warps[wid][1] = b;
+    }
     __syncthreads();
     const int t = turn++ & 1;
     if (wid == 0) {
-      v = over(warps[lane & (kThreads / 32 - 1)], kThreads / 32);
+      a = warps[lane & (kThreads / 32 - 1)][0];
+      if (two) b = warps[lane & (kThreads / 32 - 1)][1];
+      over(a, b, kThreads / 32);
       if (n == 1) {
-        if (lane == 0) slots[t][0] = v;
+        if (lane == 0) slots[t][0][0] = a;
+        if (lane == 0 && two) slots[t][1][0] = b;
       } else if (lane < n) {
-        st_cluster_v4(mapa_shared(smem_u32(&slots[t][rank]), lane), __float_as_uint(v.x), __float_as_uint(v.y),
-                      __float_as_uint(v.z), __float_as_uint(v.w));
+        auto send = [&](float4* to, const float4& v) {
+          st_cluster_v4(mapa_shared(smem_u32(to), lane), __float_as_uint(v.x), __float_as_uint(v.y),
+                        __float_as_uint(v.z), __float_as_uint(v.w));
+        };
+        send(&slots[t][0][rank], a);
+        if (two) send(&slots[t][1][rank], b);
       }
     }
     if (n == 1) __syncthreads();
     else cluster_sync();
-    v = slots[t][lane & (n - 1)];
-    return n == 1 ? v : over(v, n);
+    a = slots[t][0][lane & (n - 1)];
+    if (two) b = slots[t][1][lane & (n - 1)];
+    if (n > 1) over(a, b, n);
   }
-  // (maximum, sum of 2^((l - maximum) k))
-  CB_DEVICE float2 stat(float m, float s, float k) {
-    const float4 r = reduce(make_float4(m, s, 0.f, 0.f), [&](float4 v, int w) {
-      float top = v.x;
-      for (int o = w >> 1; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
-      float sum = v.y * ex2v((v.x - (top == -INFINITY ? 0.f : top)) * k);
-      for (int o = w >> 1; o; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
-      return make_float4(top, sum, 0.f, 0.f);
-    });
-    return make_float2(r.x, r.y);
+  // the better of (x, i) and (ox, oi): larger value, lower index among equals (index -1: none)
+  CB_DEVICE static void take(float& x, float& i, float ox, float oi) {
+    const int p = __float_as_int(i), q = __float_as_int(oi);
+    if (q >= 0 && (p < 0 || ox > x || (ox == x && q < p))) { x = ox; i = oi; }
   }
-  // maxima of the scores .x and .z and their lowest indices .y, .w (-1: none)
-  CB_DEVICE float4 best2(float4 a) {
-    return reduce(a, [](float4 v, int w) {
-      auto take = [](float& x, float& i, float ox, float oi) {
-        const int p = __float_as_int(i), q = __float_as_int(oi);
-        if (q >= 0 && (p < 0 || ox > x || (ox == x && q < p))) { x = ox; i = oi; }
-      };
+  // a: two rows' (maximum, sum of 2^((l - maximum) k)); b (greedy): their (maximum, its lowest index)
+  CB_DEVICE void stat2(float4& a, float4& b, bool greedy, float k) {
+    reduce(a, b, greedy, [&](float4& v, float4& y, int w) {
+      float m = v.x, n = v.z;
       for (int o = w >> 1; o; o >>= 1) {
-        const float4 y = make_float4(__shfl_xor_sync(~0u, v.x, o), __shfl_xor_sync(~0u, v.y, o),
-                                     __shfl_xor_sync(~0u, v.z, o), __shfl_xor_sync(~0u, v.w, o));
-        take(v.x, v.y, y.x, y.y);
-        take(v.z, v.w, y.z, y.w);
+        m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
+        n = fmaxf(n, __shfl_xor_sync(~0u, n, o));
       }
-      return v;
+      float s = v.y * ex2v((v.x - (m == -INFINITY ? 0.f : m)) * k), t = v.w * ex2v((v.z - (n == -INFINITY ? 0.f : n)) * k);
+      for (int o = w >> 1; o; o >>= 1) {
+        s += __shfl_xor_sync(~0u, s, o);
+        t += __shfl_xor_sync(~0u, t, o);
+      }
+      v = make_float4(m, s, n, t);
+      if (greedy) best(y, w);
     });
   }
-  CB_DEVICE float sum(float a) {
-    return reduce(make_float4(a, 0.f, 0.f, 0.f), [](float4 v, int w) {
+  CB_DEVICE static void best(float4& v, int w) {
+    for (int o = w >> 1; o; o >>= 1) {
+      const float4 y = make_float4(__shfl_xor_sync(~0u, v.x, o), __shfl_xor_sync(~0u, v.y, o),
+                                   __shfl_xor_sync(~0u, v.z, o), __shfl_xor_sync(~0u, v.w, o));
+      take(v.x, v.y, y.x, y.y);
+      take(v.z, v.w, y.z, y.w);
+    }
+  }
+  // maxima of the scores .x and .z and their lowest indices .y, .w
+  CB_DEVICE float4 best2(float4 a) {
+    float4 none = a;
+    reduce(a, none, false, [](float4& v, float4&, int w) { best(v, w); });
+    return a;
+  }
+  CB_DEVICE float sum(float x) {
+    float4 a = make_float4(x, 0.f, 0.f, 0.f), none = a;
+    reduce(a, none, false, [](float4& v, float4&, int w) {
       for (int o = w >> 1; o; o >>= 1) v.x += __shfl_xor_sync(~0u, v.x, o);
-      return v;
-    }).x;
+    });
+    return a.x;
   }
 };
 
-// One cluster per request: its CTAs share the vocabulary.  A visited node costs one pass over its logits; a rejection
+// One cluster per request: its CTAs share the vocabulary.  A visited node costs one pass over its logits (while requests
+// are too few to fill HBM, a pass takes the node's first child along: most are accepted, and then need none); a rejection
 // of a token drawn from a distribution one pass over logits and distribution for the remainder's sum (not needed for
 // the last child, whose remainder goes straight into the draw); the end one pass over logits, distribution and noise.
 template <bool BF16, bool DRAFT>
@@ -92,9 +115,10 @@ __global__ void __launch_bounds__(kThreads, 2) tree_verify_kernel(
     const float* __restrict__ temperature, const float* __restrict__ draft, int clusters, int* __restrict__ path,
     int* __restrict__ n_accepted, int* __restrict__ out_tokens, float* __restrict__ logprobs) {
   pdl_entry();
-  __shared__ float4 sh_slots[2][kMaxCluster], sh_warps[kThreads / 32];
+  __shared__ float4 sh_slots[2][2][kMaxCluster], sh_warps[kThreads / 32][2];
   __shared__ int s_tok[kNodes], s_par[kNodes], s_child[kNodes], s_sib[kNodes], s_gone[kNodes];
   __shared__ float s_u[kNodes], s_l[kNodes], s_q[kNodes], s_mass[kNodes];
+  __shared__ float4 s_stat;                            // of the first child: maximum, sum, index of the maximum
   const int n_cta = gridDim.x / clusters;
   const int rank = n_cta == 1 ? 0 : int(cluster_ctarank()), b = blockIdx.x / n_cta;
   Exchange ex{sh_slots, sh_warps, n_cta, rank, 0};
@@ -129,51 +153,84 @@ __global__ void __launch_bounds__(kThreads, 2) tree_verify_kernel(
   const float k = greedy ? kLog2e : kLog2e / T;        // p = 2^((l - max) k) / total
   const int per = (V + n_cta - 1) / n_cta, lo = rank * per, hi = min(V, lo + per);
   const float* e = noise + size_t(b) * V;
-  int v = 0, steps = 0;
+  auto row_of = [&](int node) {
+    return reinterpret_cast<const char*>(logits) + (size_t(t0 + node) * ld) * (BF16 ? 2 : 4);
+  };
+  auto at = [](const char* row, int i) -> float {
+    if constexpr (BF16) return __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(row)[i]);
+    else return reinterpret_cast<const float*>(row)[i];
+  };
+  int v = 0, steps = 0, known = -1;                    // known: the node whose statistics are in s_stat
   while (true) {
-    const char* rowp = reinterpret_cast<const char*>(logits) + (size_t(t0 + v) * ld) * (BF16 ? 2 : 4);
+    const char* rowp = row_of(v);
     const float* q = DRAFT ? draft + size_t(t0 + v) * V : nullptr;
-    auto logit = [&](int i) -> float {
-      if constexpr (BF16) return __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(rowp)[i]);
-      else return reinterpret_cast<const float*>(rowp)[i];
-    };
-    // the children's logits and draft probabilities, read while the pass runs
-    if (int(threadIdx.x) < n && s_par[threadIdx.x] == v) {
-      const int x = s_tok[threadIdx.x];
-      const bool in = x >= 0 && x < V;
-      s_l[threadIdx.x] = in ? logit(x) : -INFINITY;
-      s_q[threadIdx.x] = in ? (DRAFT ? q[x] : 1.f) : -1.f;      // no such token: never accepted
-    }
-    float m = -INFINITY, s = 0.f;
-    int at = -1;
-    for (int i0 = lo + int(threadIdx.x); i0 < hi; i0 += kThreads * kWide) {
-      float x[kWide], top = m;
+    auto logit = [&](int i) { return at(rowp, i); };
+    float4 st;                                         // maximum, sum, index of the maximum (greedy)
+    if (v == known) {
+      st = s_stat;
+    } else {
+      const int w = n_cta > 1 ? s_child[v] : -1;       // taken along
+      const char* roww = w >= 0 ? row_of(w) : rowp;
+      // the children's logits and draft probabilities, read while the pass runs
+      if (int(threadIdx.x) < n) {
+        const int up = s_par[threadIdx.x], x = s_tok[threadIdx.x];
+        if (up == v || (up == w && w >= 0)) {
+          const bool in = x >= 0 && x < V;
+          s_l[threadIdx.x] = in ? at(row_of(up), x) : -INFINITY;
+          s_q[threadIdx.x] = in ? (DRAFT ? draft[size_t(t0 + up) * V + x] : 1.f) : -1.f;   // no such token: never accepted
+        }
+      }
+      float m[2] = {-INFINITY, -INFINITY}, s[2] = {0.f, 0.f};
+      int best[2] = {-1, -1};
+      auto fold = [&](int r, const float* x, int cnt, int i0) {
+        float top = m[r];
+        if (greedy) {
+          if (best[r] < 0) best[r] = i0;
 #pragma unroll
-      for (int u = 0; u < kWide; ++u) x[u] = i0 + u * kThreads < hi ? logit(i0 + u * kThreads) : -INFINITY;
-      if (greedy) {
-        if (at < 0) at = i0;
+          for (int u = 0; u < kWide; ++u)
+            if (u < cnt && x[u] > top) { top = x[u]; best[r] = i0 + u * kThreads; }
+        } else {
+#pragma unroll
+          for (int u = 0; u < kWide; ++u)
+            if (u < cnt) top = fmaxf(top, x[u]);
+        }
+        const float ref = top == -INFINITY ? 0.f : top;
+        s[r] *= ex2v((m[r] - ref) * k);
 #pragma unroll
         for (int u = 0; u < kWide; ++u)
-          if (x[u] > top) { top = x[u]; at = i0 + u * kThreads; }
+          if (u < cnt) s[r] += ex2v((x[u] - ref) * k);
+        m[r] = top;
+      };
+      if (w < 0) {                                     // sixteen loads in flight
+        for (int i0 = lo + int(threadIdx.x); i0 < hi; i0 += kThreads * kWide) {
+          float x[kWide];
+#pragma unroll
+          for (int u = 0; u < kWide; ++u) x[u] = i0 + u * kThreads < hi ? logit(i0 + u * kThreads) : -INFINITY;
+          fold(0, x, kWide, i0);
+        }
       } else {
+        for (int i0 = lo + int(threadIdx.x); i0 < hi; i0 += kThreads * kUnroll) {
+          float x[kUnroll], y[kUnroll];
 #pragma unroll
-        for (int u = 0; u < kWide; ++u) top = fmaxf(top, x[u]);
+          for (int u = 0; u < kUnroll; ++u) {
+            const int i = i0 + u * kThreads;
+            x[u] = i < hi ? logit(i) : -INFINITY;
+            y[u] = i < hi ? at(roww, i) : -INFINITY;
+          }
+          fold(0, x, kUnroll, i0);
+          fold(1, y, kUnroll, i0);
+        }
       }
-      const float ref = top == -INFINITY ? 0.f : top;
-      s *= ex2v((m - ref) * k);
-#pragma unroll
-      for (int u = 0; u < kWide; ++u) s += ex2v((x[u] - ref) * k);
-      m = top;
+      float4 both = make_float4(m[0], s[0], m[1], s[1]);
+      float4 idx = make_float4(m[0], __int_as_float(best[0]), m[1], __int_as_float(best[1]));
+      ex.stat2(both, idx, greedy, k);
+      st = make_float4(both.x, both.y, idx.y, 0.f);
+      if (threadIdx.x == 0) s_stat = make_float4(both.z, both.w, idx.w, 0.f);   // read after the walk's next barrier
+      known = w;
     }
-    const float mine = m;
-    const float2 st = ex.stat(m, s, k);
     const float ref = st.x == -INFINITY ? 0.f : st.x, total = st.y;
     const float inv = total > 0.f ? 1.f / total : (total == total ? 0.f : total);
-    int best = -1;                                     // greedy: the lowest-index maximum
-    if (greedy) {
-      best = __float_as_int(ex.best2(make_float4(mine, __int_as_float(at), 0.f, __int_as_float(-1))).y);
-      if (!(total > 0.f)) best = -1;
-    }
+    const int best = total > 0.f ? __float_as_int(st.z) : -1;
     const float lse = log2f(total);
     auto logprob = [&](float l) { return ((l - ref) * k - lse) * 0.6931471805599453f; };
     int gone = 0;                                      // rejections that changed the remainder
@@ -246,22 +303,23 @@ __global__ void __launch_bounds__(kThreads, 2) tree_verify_kernel(
       // rejection, which stands if that left nothing.
       float r1 = 0.f, e1 = 1.f, r0 = 0.f, e0 = 1.f;
       int w1 = -1, w0 = -1;
+      const bool with_q = DRAFT && (open || gone > 0);  // else the distribution is not read
       for (int i0 = lo + int(threadIdx.x); i0 < hi; i0 += kThreads * kUnroll) {
         float r[kUnroll], qi[kUnroll], ei[kUnroll];
 #pragma unroll
         for (int u = 0; u < kUnroll; ++u) {
           const int i = i0 + u * kThreads;
           r[u] = i < hi ? logit(i) : -INFINITY;
-          qi[u] = DRAFT && i < hi ? q[i] : 0.f;
+          qi[u] = with_q && i < hi ? q[i] : 0.f;
           ei[u] = i < hi ? e[i] : 1.f;
         }
         rest(r, qi, i0, kUnroll);
 #pragma unroll
         for (int u = 0; u < kUnroll; ++u) {
           const int i = i0 + u * kThreads;
-          if (DRAFT && r[u] * e0 > r0 * ei[u]) { r0 = r[u]; e0 = ei[u]; w0 = i; }
           const float d = DRAFT && open ? fmaxf(r[u] - qi[u], 0.f) : r[u];
           if (d * e1 > r1 * ei[u]) { r1 = d; e1 = ei[u]; w1 = i; }
+          if (DRAFT && open && r[u] * e0 > r0 * ei[u]) { r0 = r[u]; e0 = ei[u]; w0 = i; }
         }
       }
       const float4 w = ex.best2(make_float4(r1 / e1, __int_as_float(w1), r0 / e0, __int_as_float(w0)));
