@@ -142,21 +142,37 @@ int tree_mla(const Tensor& q, const Tensor& kv, const Tensor& cu, const Tensor& 
                       part, part ? part + counts[3] * 128 * 512 : nullptr, ptr<void>(staged), ptr<int>(status), out.data_ptr(), stream());
 }
 
-// out: int32 [B (2 N + 1)] = path [B, N], n_accepted [B], tokens [B, N], returned as views
-std::tuple<int, Tensor, Tensor, Tensor> tree_verify(const Tensor& logits, const Tensor& tokens, const Tensor& cu,
-                                                    const Tensor& parent, int64_t N, const Tensor& uniforms,
-                                                    const Tensor& noise, const Tensor& temperature,
-                                                    const OptTensor& draft, const Tensor& out,
-                                                    const Tensor& logprobs) {
-  c10::cuda::CUDAGuard g(logits.device());
-  const int64_t B = cu.numel() - 1;
+// Whether t is a contiguous tensor of this type, size and device.
+bool fits(const Tensor& t, at::ScalarType dt, const c10::Device& dev, std::initializer_list<int64_t> shape) {
+  return t.scalar_type() == dt && t.device() == dev && t.is_contiguous() && t.sizes().equals(shape);
+}
+
+// out: int32 [B (3 N + 1)] = path [B, N], n_accepted [B], tokens [B, N], logprobs [B, N] (fp32), returned as views.
+// Code -1: an argument does not fit (the caller says which).
+std::tuple<int, Tensor, Tensor, Tensor, Tensor> tree_verify(const Tensor& logits, const Tensor& tokens,
+                                                            const Tensor& cu, const Tensor& parent, int64_t N,
+                                                            const Tensor& uniforms, const Tensor& noise,
+                                                            const Tensor& temperature, const OptTensor& draft,
+                                                            const Tensor& out) {
+  const c10::Device dev = cu.device();
+  const int64_t B = cu.numel() - 1, T = parent.numel();
+  const bool bf16 = logits.scalar_type() == at::kBFloat16;
+  bool ok = logits.dim() == 2 && logits.size(0) == T && (bf16 || logits.scalar_type() == at::kFloat) &&
+            logits.device() == dev;
+  const int64_t V = ok ? logits.size(1) : 0;
+  ok = ok && V > 0 && V < (int64_t(1) << 31) && (T == 0 || logits.stride(1) == 1) &&
+       fits(tokens, at::kInt, dev, {T}) && fits(uniforms, at::kFloat, dev, {T}) &&
+       fits(noise, at::kFloat, dev, {B, V}) && fits(temperature, at::kFloat, dev, {B}) &&
+       (!draft.has_value() || fits(*draft, at::kFloat, dev, {T, V}));
+  if (!ok) return {-1, out, out, out, out};
+  c10::cuda::CUDAGuard g(dev);
   int* o = ptr<int>(out);
-  const int e = cb::tree_verify(logits.data_ptr(), logits.scalar_type() == at::kBFloat16, logits.stride(0),
-                                int(logits.size(1)), ptr<int>(tokens), ptr<int>(cu), ptr<int>(parent), int(B), int(N),
-                                ptr<float>(uniforms), ptr<float>(noise), ptr<float>(temperature), ptr<float>(draft),
-                                o, o + B * N, o + B * (N + 1), ptr<float>(logprobs), stream());
+  const int e = cb::tree_verify(logits.data_ptr(), bf16, logits.stride(0), int(V), ptr<int>(tokens), ptr<int>(cu),
+                                ptr<int>(parent), int(B), int(N), ptr<float>(uniforms), ptr<float>(noise),
+                                ptr<float>(temperature), ptr<float>(draft), o, o + B * N, o + B * (N + 1),
+                                reinterpret_cast<float*>(o + B * (2 * N + 1)), stream());
   return {e, out.as_strided({B, N}, {N, 1}, 0), out.as_strided({B}, {1}, B * N),
-          out.as_strided({B, N}, {N, 1}, B * (N + 1))};
+          out.as_strided({B, N}, {N, 1}, B * (N + 1)), out.view(at::kFloat).as_strided({B, N}, {N, 1}, B * (2 * N + 1))};
 }
 
 int tree_commit(const Tensor& caches, int64_t max_row, bool wide, const Tensor& cu, const Tensor& ctx,

@@ -221,6 +221,28 @@ class TreeVerdict(NamedTuple):
     logprobs: torch.Tensor
 
 
+def _check_verify(logits, tokens, plan, uniforms, noise, temperature, draft_probs) -> None:
+    """Raise for the first argument of tree_verify that does not fit."""
+    T, B, V = plan.T, plan.B, logits.shape[-1]
+    for name, t, shape in (("logits", logits, (T, V)), ("tokens", tokens, (T,)), ("uniforms", uniforms, (T,)),
+                           ("noise", noise, (B, V)), ("temperature", temperature, (B,)),
+                           ("draft_probs", draft_probs, (T, V))):
+        if t is not None and t.shape != shape:
+            raise ValueError(f"tree_verify: {name} has shape {tuple(t.shape)}, expected {shape}")
+    if logits.device != plan.device:
+        raise ValueError(f"tree_verify: logits are on {logits.device}, the plan on {plan.device}")
+    if plan.device.type != "cuda":
+        return
+    if logits.dtype not in (torch.float32, torch.bfloat16) or not 0 < V < 1 << 31 or (T and logits.stride(1) != 1):
+        raise ValueError(f"tree_verify: logits must be fp32 or bf16 with a unit column stride, got {logits.dtype}, "
+                         f"strides {logits.stride()}")
+    for name, t, dtype in (("tokens", tokens, torch.int32), ("uniforms", uniforms, torch.float32),
+                           ("noise", noise, torch.float32), ("temperature", temperature, torch.float32),
+                           ("draft_probs", draft_probs, torch.float32)):
+        if t is not None:
+            _need(f"tree_verify: {name}", t, plan.device.index, dtype)
+
+
 def tree_verify(logits: torch.Tensor, tokens: torch.Tensor, plan: TreePlan, uniforms: torch.Tensor,
                 noise: torch.Tensor, temperature: torch.Tensor, draft_probs: Optional[torch.Tensor] = None
                 ) -> TreeVerdict:
@@ -230,31 +252,16 @@ def tree_verify(logits: torch.Tensor, tokens: torch.Tensor, plan: TreePlan, unif
     greedy); draft_probs [T, V] fp32: row t = the distribution that node t's children were drawn from (independent
     draws), None = certain proposals (prompt lookup, a draft model's best tokens).  The emitted tokens are distributed
     as the target's own samples."""
-    T, B, V = plan.T, plan.B, logits.shape[1]
-    for name, t, shape in (("logits", logits, (T, V)), ("tokens", tokens, (T,)), ("uniforms", uniforms, (T,)),
-                           ("noise", noise, (B, V)), ("temperature", temperature, (B,)),
-                           ("draft_probs", draft_probs, (T, V))):
-        if t is not None and t.shape != shape:
-            raise ValueError(f"tree_verify: {name} has shape {tuple(t.shape)}, expected {shape}")
-    N = plan.N
-    if logits.is_cuda:
-        dev = plan.device.index
-        if logits.get_device() != dev or logits.dtype not in (torch.float32, torch.bfloat16) or not 0 < V < 1 << 31 or (
-                T and logits.stride(1) != 1):
-            raise ValueError(f"tree_verify: logits must be fp32 or bf16 on {plan.device} with a unit column stride, "
-                             f"got {logits.dtype} on {logits.device}, strides {logits.stride()}")
-        _need("tree_verify: tokens", tokens, dev, torch.int32)
-        _need("tree_verify: uniforms", uniforms, dev, torch.float32)
-        _need("tree_verify: noise", noise, dev, torch.float32)
-        _need("tree_verify: temperature", temperature, dev, torch.float32)
-        if draft_probs is not None:
-            _need("tree_verify: draft_probs", draft_probs, dev, torch.float32)
-        out = torch.empty(B * (2 * N + 1), dtype=torch.int32, device=logits.device)
-        lp = torch.empty(B, N, dtype=torch.float32, device=logits.device)
-        code, path, n, toks = ext().tree_verify(logits, tokens, plan.cu, plan.parent, N, uniforms, noise, temperature,
-                                                draft_probs, out, lp)
+    B, N = plan.B, plan.N
+    if logits.is_cuda and plan.device.type == "cuda":
+        out = torch.empty(B * (3 * N + 1), dtype=torch.int32, device=plan.device)
+        code, path, n, toks, lp = ext().tree_verify(logits, tokens, plan.cu, plan.parent, N, uniforms, noise,
+                                                    temperature, draft_probs, out)
+        if code == -1:
+            _check_verify(logits, tokens, plan, uniforms, noise, temperature, draft_probs)
         _launched(code, "tree_verify")
         return TreeVerdict(path, n, toks, lp)
+    _check_verify(logits, tokens, plan, uniforms, noise, temperature, draft_probs)
     v = TreeVerdict(torch.full((B, N), -1, dtype=torch.int32), torch.full((B,), -1, dtype=torch.int32),
                     torch.full((B, N), -1, dtype=torch.int32), torch.zeros(B, N))
     for b in range(B):
