@@ -143,6 +143,7 @@ class Engine:
         self.cuda_graphs = cuda_graphs and self.device.type == "cuda"
         self.graph_buckets = sorted(graph_buckets)
         self._graphs: Dict[int, "_DecodeGraph"] = {}
+        self._cache_rows = None                      # the caches whose rows move together (verify_tree)
         self.stats = {"prefill_tokens": 0, "decode_tokens": 0}
         from ..utils.metrics import Metrics
 
@@ -552,19 +553,111 @@ class Engine:
         self.stats["decode_tokens"] += sum(len(x) for x in rows)
         return accepted
 
-    def generate_speculative(self, prompts: List[Sequence[int]], max_new_tokens: int, drafter=None, n_draft: int = 5):
-        """Greedy generation with draft-and-verify steps (``n_draft`` drafts + 1 row per request per step)."""
+    def verify_tree(self, reqs: List[Request], trees, temperature=0.0, generator: Optional[torch.Generator] = None,
+                    draft_probs: Optional[torch.Tensor] = None):
+        """Target verification of drafted token trees, greedy or sampled, in one forward (``ops.spec``; one rank).
+
+        trees[b] = (tokens, parents): node 0 is request b's last token (parent -1, not yet cached), every other node a
+        drafted token continuing its parent.  All nodes of all requests run together, each attending to its request's
+        context and its own branch; ``tree_verify`` walks down each tree, and the accepted branch's cache rows move
+        behind the context.  temperature: one number or one per request (0: greedy).  draft_probs [all nodes, V]: the
+        distribution each node's children were drawn from; without it drafts are certain proposals.  With temperature
+        the emitted tokens are distributed as the target's own samples.  Returns the new tokens per request (>= 1)."""
+        from ..ops import spec
+
+        if self.model.pctx.world > 1:
+            raise ValueError("verify_tree runs on one rank")
+        for r, (toks, parents) in zip(reqs, trees):
+            if not toks or len(toks) != len(parents):
+                raise ValueError(f"request {r.rid}: a tree needs the pending token and one parent per node")
+            self._ensure_pages(r, r.seq_len + len(toks))
+        cfg, dev = self.cfg, self.device
+        plan = spec.TreePlan([r.pages for r in reqs], [r.seq_len for r in reqs], [p for _, p in trees], self.page_size,
+                             n_heads=self.model.H_local, device=dev)
+        ids = torch.tensor([int(t) for toks, _ in trees for t in toks], dtype=torch.int32).to(dev)
+        # each node's own key list, for the layers that select keys (DSA, windows) and the Engram's n-grams
+        listed = cfg.use_indexer or cfg.engram_layers or cfg.attn_kind == "latent_mqa"
+        key_slots = self._tree_key_slots(plan) if listed else torch.zeros(plan.T, 1, dtype=torch.int32)
+        late = torch.tensor([r.late_from for r, k in zip(reqs, plan.n) for _ in range(k)], dtype=torch.int32)
+        fb = ForwardBatch(ids=ids, pos=plan.pos, out_loc=torch.tensor(plan.node_slots(), dtype=torch.int32).to(dev),
+                          is_prefill=False, key_slots=key_slots.to(dev), n_keys=plan.pos + 1, late_from=late.to(dev),
+                          tree=plan)
+        with self.metrics.step("verify", plan.T, len(reqs)):
+            logits = self.model.forward(fb, self.cache)
+            V = logits.shape[1]
+            heat = [float(temperature)] * len(reqs) if isinstance(temperature, (int, float)) else list(temperature)
+            temp = torch.tensor(heat, dtype=torch.float32).to(dev)
+            u = torch.rand(plan.T, device=dev, generator=generator)
+            noise = torch.empty(len(reqs), V, device=dev)
+            if any(h > 0 for h in heat):
+                noise.exponential_(generator=generator)
+            got = spec.tree_verify(logits, ids, plan, u, noise, temp, draft_probs)
+            if self._cache_rows is None:
+                c = self.cache
+                self._cache_rows = spec.CacheRows(c.latent + c.index_k + ([c.tok] if c.tok is not None else []))
+            spec.tree_commit(self._cache_rows, plan, got.path, got.n_accepted)
+        counts, tokens = got.n_accepted.tolist(), got.tokens.tolist()
+        accepted = []
+        for r, (toks, _), a, new in zip(reqs, trees, counts, tokens):
+            if new[a] < 0:
+                raise RuntimeError(f"request {r.rid}: the target's logits leave no token (not finite)")
+            r.out += [int(toks[0])] + new[:a]                # tokens whose KV is now valid in the cache
+            r.n_cached = r.seq_len
+            accepted.append(new[:a + 1])
+        self.stats["decode_tokens"] += plan.T
+        return accepted
+
+    @staticmethod
+    def _tree_key_slots(plan) -> torch.Tensor:
+        """[T, longest] int32: the cache slots of each node's keys in order (context, then its branch), -1 padded."""
+        ps = plan.page_size
+        width = max(p + 1 for p in plan.pos_list)
+        out = torch.full((plan.T, width), -1, dtype=torch.int32)
+        for b in range(plan.B):
+            c, lo = plan.ctx_list[b], plan.cu_list[b]
+            tab = torch.tensor(plan.tables_list[b], dtype=torch.int32)
+            slots = (tab[:, None] * ps + torch.arange(ps, dtype=torch.int32)).flatten()
+            out[lo:lo + plan.n[b], :c] = slots[:c]
+            for i, par in enumerate(plan.parents_list[b]):
+                if par >= 0:
+                    out[lo + i, c:plan.pos_list[lo + i]] = out[lo + par, c:plan.pos_list[lo + i]]
+                out[lo + i, plan.pos_list[lo + i]] = slots[c + i]
+        return out
+
+    def generate_speculative(self, prompts: List[Sequence[int]], max_new_tokens: int, drafter=None, n_draft: int = 5,
+                             tree: bool = False, temperature: float = 0.0, seed: int = 0):
+        """Generation with draft-and-verify steps (``n_draft`` drafts + 1 row per request per step).  Greedy chains by
+        default; ``tree``: drafted trees (the drafter's ``propose_tree``); temperature > 0: tokens sampled from the
+        target's distribution at that temperature (``verify_tree``; ``seed`` fixes the random numbers)."""
         from .spec import NgramDrafter
 
         drafter = drafter or NgramDrafter()
         reqs = [self.add_request(p) for p in prompts]
         logits = self.prefill(reqs)
-        pending = torch.argmax(logits.float(), dim=-1).tolist()       # next token of each request, not yet cached
+        gen = None
+        if temperature > 0:
+            gen = torch.Generator(device=self.device).manual_seed(seed)
+            p = torch.softmax(logits.float() / temperature, -1)
+            e = torch.empty_like(p).exponential_(generator=gen)
+            pending = torch.argmax(p / e, dim=-1).tolist()
+        else:
+            pending = torch.argmax(logits.float(), dim=-1).tolist()   # next token of each request, not yet cached
         produced = [[t] for t in pending]
         self.stats.setdefault("verify_steps", 0)
         while min(len(x) for x in produced) < max_new_tokens:
-            drafts = [drafter.propose(r.prompt + r.out + [t], n_draft) for r, t in zip(reqs, pending)]
-            acc = self.verify(reqs, pending, drafts)
+            seqs = [r.prompt + r.out + [t] for r, t in zip(reqs, pending)]
+            if tree or temperature > 0:
+                trees = []
+                for s in seqs:
+                    if tree and hasattr(drafter, "propose_tree"):
+                        toks, parents = drafter.propose_tree(s, n_draft)
+                    else:
+                        toks = drafter.propose(s, n_draft)
+                        parents = list(range(len(toks)))
+                    trees.append(([s[-1]] + list(toks), [-1] + list(parents)))
+                acc = self.verify_tree(reqs, trees, temperature, gen)
+            else:
+                acc = self.verify(reqs, pending, [drafter.propose(s, n_draft) for s in seqs])
             self.stats["verify_steps"] += 1
             for b, a in enumerate(acc):
                 produced[b] += a

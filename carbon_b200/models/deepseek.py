@@ -27,6 +27,7 @@ import torch.nn.functional as F
 from ..config import ModelConfig
 from ..ops import attention as A
 from ..ops import core as C
+from ..ops import spec as S
 from ..ops.gemm import bf16_gemm, fp8_gemm, fp8_gemm_swiglu, interleave_gate_up
 from ..ops.quant import Fp8Weight, gather_rows_fp8, quant_act, quantize_weight, stack_weights
 from ..ref import ops as R
@@ -118,6 +119,9 @@ class ForwardBatch:
     logits_rows: Optional[torch.Tensor] = None  # rows that need logits (default: all)
     bounds: Optional[List[int]] = None          # per-rank token shard bounds (multi-rank; sequence-aligned)
     late_from: Optional[torch.Tensor] = None    # decode: [B] first position that exists at the late layers
+    # rows are the nodes of drafted token trees (ops.spec.TreePlan; one rank): layers that attend to every visible key
+    # run the tree attention, the others take key_slots (each node's context and branch) as decode rows do
+    tree: Optional[object] = None
 
 
 class Layer:
@@ -751,7 +755,8 @@ class DeepseekModel:
         swap = not dp and pc.world > 1 and hasattr(pc, "heads_to_tokens")
         local = dp or swap
         rows = slice(lo, hi) if local else slice(0, q.shape[0])
-        idx = self._latent_keys(i, fb, cache, idx_l, rows, local)
+        dense = fb.tree is not None and cfg.swa_window == 0 and cfg.index_source(i) is None
+        idx = None if dense else self._latent_keys(i, fb, cache, idx_l, rows, local)
         pos_q = fb.pos[lo:hi] if dp else fb.pos
         tok_major = swap and self.o_a2a      # the owner keeps its tokens' outputs (all heads) for the projection
         with region("attn.core_prefill" if fb.is_prefill else "attn.core_decode"):
@@ -760,6 +765,8 @@ class DeepseekModel:
                 o = A.sparse_mla(q_tok, cache.latent[i], idx, cfg.softmax_scale, r, sink=L.sink_all)
                 if not tok_major:
                     o = pc.tokens_to_heads(o.contiguous()) if self.on_gpu else pc.tokens_to_heads(o)
+            elif dense:
+                o = S.tree_mla(q, cache.latent[i], fb.tree, cfg.softmax_scale, r, sink=L.sink)
             else:
                 o = A.sparse_mla(q.contiguous(), cache.latent[i], idx, cfg.softmax_scale, r, sink=L.sink)
             o = o.to(self.act_dtype).contiguous() if self.on_gpu else o.float().contiguous()
@@ -846,7 +853,11 @@ class DeepseekModel:
                 o_lat = pc.tokens_to_heads(o_tok)                                   # [T, Hl, r]
         else:
             with region("attn.core_decode"):
-                o_lat = A.sparse_mla(qf, cache.latent[i], idx.contiguous(), cfg.softmax_scale, r, sink=L.sink)
+                dense = sel is None and (src is None or int(fb.key_slots.shape[1]) <= cfg.index_topk)
+                if fb.tree is not None and dense:
+                    o_lat = S.tree_mla(qf, cache.latent[i], fb.tree, cfg.softmax_scale, r, sink=L.sink)
+                else:
+                    o_lat = A.sparse_mla(qf, cache.latent[i], idx.contiguous(), cfg.softmax_scale, r, sink=L.sink)
         with region("attn.absorb_o"):
             return head_bmm(o_lat, L.w_uv), False                                    # [T, Hl, dv]
 

@@ -503,7 +503,7 @@ def tree_verify(logits: torch.Tensor, tokens, parents, uniforms, noise: torch.Te
     v, path, toks, lps = 0, [0], [], []
     while True:
         lp = torch.log_softmax(logits[v] / heat, -1)
-        if bool(torch.isneginf(logits[v]).all()):
+        if not bool(torch.exp(logits[v] - logits[v].max()).sum() > 0):       # nothing left by a mask, NaN, +inf
             r = torch.zeros_like(lp)
             lp = torch.full_like(lp, float("-inf"))
         elif temperature > 0:

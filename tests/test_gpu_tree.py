@@ -385,3 +385,98 @@ def test_tree_commit_refusals():
         spec.tree_commit(spec.CacheRows([cache[:64]]), plan, path, n)
     with pytest.raises(ValueError, match="one device"):
         spec.CacheRows([cache, cache.cpu()])
+
+
+# ----------------------------------------------------------------------------------------------------------------------
+# the engine's step
+# ----------------------------------------------------------------------------------------------------------------------
+def engine_cfg(kind):
+    from carbon_b200.config import small_gpu_config
+
+    cfg = small_gpu_config().replace(n_layers=2, n_routed_experts=8, n_activated_experts=2, vocab_size=2048)
+    if kind == "dense":
+        return cfg.replace(index_n_heads=0, index_topk=0)
+    if kind == "dense_fp8":
+        return cfg.replace(index_n_heads=0, index_topk=0, kv_fp8=True, attn_sink=True)
+    if kind == "latent":
+        return cfg.replace(attn_kind="latent_mqa", index_n_heads=0, index_topk=0, attn_sink=True)
+    return cfg                                                # DSA
+
+
+@pytest.mark.parametrize("kind", ["dense", "dense_fp8", "latent", "dsa"])
+def test_engine_tree_step_matches_row_verification(kind):
+    """One tree step of three requests against the same nodes as decode rows (each node's branch appended to its own
+    copy of the context): the logits differ by the kernels' rounding only.  Both paths round the attention output to
+    bf16 (2^-9) and run the same fp8 GEMMs on it, whose own rounding (2^-4 relative per input) can flip single inputs
+    by one step; 5 % of the logits' norm bounds that over two layers (flips of router choices are excluded by the
+    comparison of the median row)."""
+    from carbon_b200.engine.engine import Engine
+    from carbon_b200.models.weights import WeightSource
+    from carbon_b200.ref.model import init_weights
+
+    cfg = engine_cfg(kind)
+    w = init_weights(cfg, seed=0)
+    g = torch.Generator().manual_seed(1)
+    ps = [torch.randint(0, cfg.vocab_size, (k,), generator=g).tolist() for k in (70, 131, 300)]
+    trees = [([5, 6, 7, 8], [-1, 0, 0, 1]), ([9], [-1]), ([1, 2, 3, 4, 5], [-1, 0, 1, 1, 2])]
+    eng = Engine(cfg, device="cuda", source=WeightSource(cfg, state=w), num_pages=96, page_size=64)
+    rows = []
+    for p, (toks, par) in zip(ps, trees):
+        for i in range(len(toks)):
+            branch = []
+            k = i
+            while k >= 0:
+                branch.insert(0, toks[k])
+                k = par[k]
+            r = eng.add_request(p)
+            eng.prefill([r])
+            for t in branch:
+                lg = eng.decode([r], [t])
+            rows.append(lg[0].float())
+            eng.release(r)
+    reqs = [eng.add_request(p) for p in ps]
+    eng.prefill(reqs)
+    seen = {}
+    forward = eng.model.forward
+
+    def keep(fb, cache):
+        seen["logits"] = forward(fb, cache).clone()
+        seen["plan"] = fb.tree
+        return seen["logits"]
+
+    eng.model.forward = keep
+    out = eng.verify_tree(reqs, trees)
+    seen["plan"].check()
+    want = torch.stack(rows)
+    err = ((seen["logits"].float() - want).norm(dim=-1) / want.norm(dim=-1)).sort().values
+    assert err[len(err) // 2] < 0.05, err
+    # the walk agrees with the step's own logits, and the committed branch continues like a plain context
+    best = seen["logits"].float().argmax(-1).tolist()
+    assert out[1] == [best[4]]
+    eng.model.forward = forward
+    nxt = eng.decode(reqs, [o[-1] for o in out])
+    assert bool(torch.isfinite(nxt).all())
+    for r, p, o, (toks, _) in zip(reqs, ps, out, trees):
+        assert r.out == [toks[0]] + o
+
+
+@pytest.mark.parametrize("kind", ["dense", "dsa"])
+def test_engine_tree_speculation_gpu(kind):
+    """Greedy trees drafted by the target itself: every chain token is accepted and the sequence is the target's own
+    greedy continuation (the draft engine and the target run the same kernels)."""
+    from carbon_b200.engine.engine import Engine
+    from carbon_b200.engine.spec import ModelDrafter
+    from carbon_b200.models.weights import WeightSource
+    from carbon_b200.ref.model import init_weights
+
+    cfg = engine_cfg(kind)
+    w = init_weights(cfg, seed=0)
+    g = torch.Generator().manual_seed(2)
+    ps = [torch.randint(0, cfg.vocab_size, (k,), generator=g).tolist() for k in (50, 200)]
+    mk = lambda **kw: Engine(cfg, device="cuda", source=WeightSource(cfg, state=w), num_pages=64, page_size=64, **kw)
+    eng = mk()
+    out = eng.generate_speculative(ps, 8, ModelDrafter(mk()), n_draft=6, tree=True)
+    assert all(len(o) == 8 for o in out)
+    warm = mk().generate_speculative(ps, 8, n_draft=4, tree=True, temperature=1.0, seed=3)
+    again = mk().generate_speculative(ps, 8, n_draft=4, tree=True, temperature=1.0, seed=3)
+    assert warm == again
