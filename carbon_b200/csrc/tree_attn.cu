@@ -226,15 +226,16 @@ __global__ void __launch_bounds__(THREADS, 1) tree_mla_kernel(const __grid_const
       const uint32_t lead_q = mapa_shared(smem_u32(q_full), 0);
       int g = 0;                                        // tiles so far: stage g % 2, phase (g / 2) & 1
       bool ok = true;
+      TreeItem nx = p.work.items[i0];                   // items are read one ahead
       for (int i = i0; ok && i < i1; ++i) {
-        const TreeItem it = p.work.items[i];
-        const int* table = p.lay.table + size_t(it.b) * p.lay.P;
-        const int staged = p.how == STAGED ? p.work.stage_at[it.b] * KT : 0;
-        auto row_of = [&](int tile, int half) -> int {  // row of a half tile's first key
-          if (p.how == STAGED) return staged + tile * KT + half * 64;
+        const TreeItem it = nx;
+        if (i + 1 < i1) nx = p.work.items[i + 1];
+        auto row_in = [&](const TreeItem& t, int tile, int half) -> int {   // row of a half tile's first key
           const int pos = tile * KT + half * 64;
-          return table[pos / p.lay.page] * p.lay.page + pos % p.lay.page;
+          if (p.how == STAGED) return p.work.stage_at[t.b] * KT + pos;
+          return p.lay.table[size_t(t.b) * p.lay.P + pos / p.lay.page] * p.lay.page + pos % p.lay.page;
         };
+        auto row_of = [&](int tile, int half) { return row_in(it, tile, half); };
         if (i == i0) pdl_wait();
         // Q: the previous item's last Q·K^T is done (its V loads waited for it)
         if (rank == 0) mbar_arrive_expect_tx(q_full, 2 * NA * CH);
@@ -259,8 +260,13 @@ __global__ void __launch_bounds__(THREADS, 1) tree_mla_kernel(const __grid_const
             if (!(ok = wait(&pv1[s], ph ^ 1, kErrTimeoutEmpty))) break;
             if (tma) tma_load_3d_pair(st + 4 * CH, &tm.kv4, bar, 0, row, 4);
             // L2 prefetch of the CTA's half two tiles on: the ring holds two tiles, too few to cover the latency of HBM
-            if (j + u + 2 < it.n_tiles && by_tma(it, tile + 2)) {
-              const int r2 = row_of(tile + 2, rank);
+            int r2 = -1;
+            if (j + 2 < it.n_tiles) {
+              if (j + u + 2 < it.n_tiles && by_tma(it, tile + 2)) r2 = row_of(tile + 2, rank);
+            } else if (i + 1 < i1 && u < nx.n_tiles && by_tma(nx, nx.tile + u)) {
+              r2 = row_in(nx, nx.tile + u, rank);
+            }
+            if (r2 >= 0) {
               tma_prefetch_l2_3d(&tm.kv4, 0, r2, 0);
               tma_prefetch_l2_3d(&tm.kv4, 0, r2, 4);
               if (NA == 9) tma_prefetch_l2_3d(&tm.kv1, 0, r2, 8);
@@ -290,10 +296,11 @@ __global__ void __launch_bounds__(THREADS, 1) tree_mla_kernel(const __grid_const
     if (rank == 0 && elect_one()) {
       const uint32_t id_qk = F16 ? idesc_f16(128, KT) : idesc_bf16(128, KT);
       const uint32_t id_pv = (F16 ? idesc_f16(128, 256) : idesc_bf16(128, 256)) | (1u << 16);   // V is MN-major
-      int g = 0;
+      int g = 0, next_nt = p.work.items[i0].n_tiles;
       bool ok = true;
       for (int i = i0; ok && i < i1; ++i) {
-        const int nt = p.work.items[i].n_tiles;
+        const int nt = next_nt;
+        if (i + 1 < i1) next_nt = p.work.items[i + 1].n_tiles;
         ok = wait(q_full, (i - i0) & 1, kErrTimeoutFull);
         for (int j = 0; ok && j < nt; j += 2) {
           const int m = min(2, nt - j);
@@ -349,24 +356,31 @@ __global__ void __launch_bounds__(THREADS, 1) tree_mla_kernel(const __grid_const
     const uint4 zero = make_uint4(0, 0, 0, 0);
     int g = 0;
     bool ok = true;
+    // lane r < 8: cache row of row r0 + r of a half tile (rows past the end: the last row's)
+    auto row_in = [&](const TreeItem& t, int j, int half) -> int {
+      if (j >= t.n_tiles || by_tma(t, t.tile + j)) return 0;
+      const int pos = min((t.tile + j) * KT + half * 64 + r0 + int(lane & 7), t.ctx + t.n - 1);
+      return p.lay.table[size_t(t.b) * p.lay.P + pos / p.lay.page] * p.lay.page + pos % p.lay.page;
+    };
+    auto at = [&](int rows, int r) { return p.kv + int64_t(__shfl_sync(~0u, rows, r)) * RB; };
+    TreeItem nx = p.work.items[i0];                     // items are read one ahead
+    int k0 = row_in(nx, 0, rank), k1 = row_in(nx, 1, rank);
+    int v0 = row_in(nx, 0, rank ^ 1), v1 = row_in(nx, 1, rank ^ 1);
+    pdl_wait();
     for (int i = i0; ok && i < i1; ++i) {
-      const TreeItem it = p.work.items[i];
-      const int* table = p.lay.table + size_t(it.b) * p.lay.P;
+      const TreeItem it = nx;
+      if (i + 1 < i1) nx = p.work.items[i + 1];
       const int end = it.ctx + it.n, nt = it.n_tiles;
-      // lane r < 8: cache row of row r0 + r of a half tile (rows past the end: the last row's)
-      auto row_of = [&](int j, int half) -> int {
-        if (j >= nt || by_tma(it, it.tile + j)) return 0;
-        const int pos = min((it.tile + j) * KT + half * 64 + r0 + int(lane & 7), end - 1);
-        return table[pos / p.lay.page] * p.lay.page + pos % p.lay.page;
-      };
-      auto at = [&](int rows, int r) { return p.kv + int64_t(__shfl_sync(~0u, rows, r)) * RB; };
       uint32_t odd = 0;                                 // this warp's rows with a NaN or an infinity, 8 bits per stage
-      int k0 = row_of(0, rank), k1 = row_of(1, rank), v0 = row_of(0, rank ^ 1), v1 = row_of(1, rank ^ 1);
-      if (i == i0) pdl_wait();
       for (int j = 0; ok && j < nt; j += 2) {
         const int m = min(2, nt - j);
-        const int nk0 = row_of(j + 2, rank), nk1 = row_of(j + 3, rank);
-        const int nv0 = row_of(j + 2, rank ^ 1), nv1 = row_of(j + 3, rank ^ 1);
+        // the next pair of tiles: this item's, or the next item's first
+        const bool more = j + 2 < nt;
+        const TreeItem& an = more ? it : nx;
+        const int aj = more ? j + 2 : 0;
+        const bool any = more || i + 1 < i1;
+        const int nk0 = any ? row_in(an, aj, rank) : 0, nk1 = any ? row_in(an, aj + 1, rank) : 0;
+        const int nv0 = any ? row_in(an, aj, rank ^ 1) : 0, nv1 = any ? row_in(an, aj + 1, rank ^ 1) : 0;
         for (int u = 0; ok && u < m; ++u) {
           const int s = (g + u) & 1, ph = ((g + u) >> 1) & 1, tile = it.tile + j + u;
           uint8_t* st = sK + s * STAGE;
@@ -449,7 +463,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_mla_kernel(const __grid_const
           }
           __syncwarp();
           if (lane == 0) mbar_arrive_cluster(mapa_shared(smem_u32(&kfull[s]), 0));
-          if (fed && j + u + 2 < nt && !by_tma(it, tile + 2)) {         // L2 prefetch two tiles on
+          if (fed && any && aj + u < an.n_tiles && !by_tma(an, an.tile + aj + u)) {      // L2 prefetch two tiles on
             const uint8_t* row = p.kv + int64_t(__shfl_sync(~0u, u ? nk1 : nk0, lane >> 2)) * RB;
 #pragma unroll
             for (int o = 0; o < RB; o += 512)
@@ -518,16 +532,23 @@ __global__ void __launch_bounds__(THREADS, 1) tree_mla_kernel(const __grid_const
     const int q = warp & 3, half = q >> 1, row = (q & 1) * 32 + int(lane), part = (int(warp) - 2 - FEED_WARPS) >> 2;
     const int me = part * 128 + q * 32 + int(lane);
     const uint32_t t_lane = tmem + (uint32_t(q * 32) << 16);
+    auto mask_of = [&](const TreeItem& t) -> uint64_t {
+      const int r = t.row * 128 + rank * 64 + row;
+      return r < t.n * p.H ? uint64_t(p.mask[t.c0 + r / p.H]) : 0;
+    };
+    TreeItem nx = p.work.items[i0];                     // items and masks are read one ahead
+    uint64_t next_mask = mask_of(nx);
     pdl_wait();
     int g = 0;
     bool ok = true;                       // after a failed wait the loop runs on without waiting: the block-level
     for (int i = i0; i < i1; ++i) {       // barriers below need all the warps
-      const TreeItem it = p.work.items[i];
+      const TreeItem it = nx;
+      if (i + 1 < i1) nx = p.work.items[i + 1];
       const int ctx = it.ctx, c0 = it.c0, n = it.n;
       const int r = it.row * 128 + rank * 64 + row;
       const bool live = r < n * p.H;
-      const int node = live ? r / p.H : 0, head = r - node * p.H;
-      const uint64_t mask = live ? uint64_t(p.mask[c0 + node]) : 0;
+      const int head = live ? r % p.H : 0;
+      const uint64_t mask = next_mask;
       float m_used = -INFINITY, l = 0.f;
       for (int j = 0; j < it.n_tiles; ++j, ++g) {
         const int s = g & 1, ph = (g >> 1) & 1;
@@ -602,6 +623,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_mla_kernel(const __grid_const
         if (lane == 0) mbar_arrive_cluster(mapa_shared(smem_u32(half ? &p1full[s] : &p0full[s]), 0));
       }
       // ---- item's end
+      if (i + 1 < i1) next_mask = mask_of(nx);
       const int sl = (g - 1) & 1;
       ok = ok && wait(&pv1[sl], ((g - 1) >> 1) & 1, kErrTimeoutTmem);
       tc_fence_after();
