@@ -70,6 +70,24 @@ CB_DEVICE void store32(void* p, const uint32_t* v) {      // one 32-byte sector 
                "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
                : "memory");
 }
+// Four lanes (rows) x four units of eight words: afterwards unit u of lane j is unit j of the lane u of its four.  Rows
+// that each lane holds for itself become 128-byte runs of one row over four lanes.
+CB_DEVICE void quad_transpose(uint32_t (&v)[32], int lane) {
+#pragma unroll
+  for (int step = 1; step <= 2; step *= 2) {
+    const bool up = lane & step;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      if (u & step) continue;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const uint32_t got = __shfl_xor_sync(~0u, up ? v[8 * u + k] : v[8 * (u + step) + k], step);
+        if (up) v[8 * u + k] = got;
+        else v[8 * (u + step) + k] = got;
+      }
+    }
+  }
+}
 CB_DEVICE void softmax_sync() { asm volatile("bar.sync 1, %0;" ::"n"(SM_WARPS * 32) : "memory"); }
 
 // ---------------------------------------------------------------------------------------------------------------
@@ -389,27 +407,27 @@ __global__ void __launch_bounds__(THREADS, 1) tree_mla_kernel(const __grid_const
             const int mine = u ? k1 : k0;
             const int rows = end - (tile * KT + rank * 64 + r0);        // rows of this warp that exist
             odd &= ~(0xFFu << (8 * s));
-            uint4 pe[2];                                // RoPE pieces: lane = (row of four, piece)
-            auto load_pe = [&]() {
-#pragma unroll
-              for (int k = 0; k < 2; ++k)
-                if (NA == 9) pe[k] = reinterpret_cast<const uint4*>(at(mine, 4 * k + (lane >> 3)))[(F8 ? 33 : 64) + (lane & 7)];
-            };
-            auto store_pe = [&]() {
-#pragma unroll
-              for (int k = 0; k < 2; ++k) {
-                if (NA != 9) break;
-                if (tail && 4 * k + int(lane >> 3) >= rows) pe[k] = zero;
-                put(st + 8 * CH, r0 + 4 * k + (lane >> 3), lane & 7, pe[k]);
-                if (tail) {
-                  const uint32_t bad = __ballot_sync(~0u, odd16<F8>(pe[k]));
-#pragma unroll
-                  for (int r = 0; r < 4; ++r)
-                    if ((bad >> (8 * r)) & 0xFF) odd |= 1u << (8 * s + 4 * k + r);
-                }
-              }
-            };
             if constexpr (F8) {
+              uint4 pe[2];                                // RoPE pieces: lane = (row of four, piece)
+              auto load_pe = [&]() {
+  #pragma unroll
+                for (int k = 0; k < 2; ++k)
+                  if (NA == 9) pe[k] = reinterpret_cast<const uint4*>(at(mine, 4 * k + (lane >> 3)))[33 + (lane & 7)];
+              };
+              auto store_pe = [&]() {
+  #pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                  if (NA != 9) break;
+                  if (tail && 4 * k + int(lane >> 3) >= rows) pe[k] = zero;
+                  put(st + 8 * CH, r0 + 4 * k + (lane >> 3), lane & 7, pe[k]);
+                  if (tail) {
+                    const uint32_t bad = __ballot_sync(~0u, odd16<F8>(pe[k]));
+  #pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                      if ((bad >> (8 * r)) & 0xFF) odd |= 1u << (8 * s + 4 * k + r);
+                  }
+                }
+              };
               uint4 v[8];
               uint32_t sc[8];
 #pragma unroll
@@ -434,6 +452,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_mla_kernel(const __grid_const
               }
               store_pe();
             } else {
+              uint4 pe[2];
 #pragma unroll
               for (int h = 0; h < 2; ++h) {             // four rows at a time
                 uint4 v[8];
@@ -441,21 +460,29 @@ __global__ void __launch_bounds__(THREADS, 1) tree_mla_kernel(const __grid_const
                 for (int r = 0; r < 4; ++r)
 #pragma unroll
                   for (int k = 0; k < 2; ++k) v[2 * r + k] = reinterpret_cast<const uint4*>(at(mine, 4 * h + r))[k * 32 + lane];
-                if (h == 0) {
-                  load_pe();
-                  ok = wait(&pv0[s], ph ^ 1, kErrTimeoutEmpty) && wait(&pv1[s], ph ^ 1, kErrTimeoutEmpty);
+                if (NA == 9) pe[h] = reinterpret_cast<const uint4*>(at(mine, 4 * h + (lane >> 3)))[64 + (lane & 7)];
+                if (h == 0) ok = wait(&pv0[s], ph ^ 1, kErrTimeoutEmpty) && wait(&pv1[s], ph ^ 1, kErrTimeoutEmpty);
+                if (tail) {
+#pragma unroll
+                  for (int r = 0; r < 4; ++r) {
+                    if (4 * h + r >= rows) v[2 * r] = v[2 * r + 1] = zero;
+                    if (__any_sync(~0u, odd16<F8>(v[2 * r]) || odd16<F8>(v[2 * r + 1]))) odd |= 1u << (8 * s + 4 * h + r);
+                  }
+                  if (NA == 9) {
+                    if (4 * h + int(lane >> 3) >= rows) pe[h] = zero;
+                    const uint32_t bad = __ballot_sync(~0u, odd16<F8>(pe[h]));
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                      if ((bad >> (8 * r)) & 0xFF) odd |= 1u << (8 * s + 4 * h + r);
+                  }
                 }
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                  if (tail && 4 * h + r >= rows) v[2 * r] = v[2 * r + 1] = zero;
+                for (int r = 0; r < 4; ++r)
 #pragma unroll
                   for (int k = 0; k < 2; ++k)
                     put(st + (k * 4 + (lane >> 3)) * CH, r0 + 4 * h + r, lane & 7, v[2 * r + k]);
-                  if (tail && __any_sync(~0u, odd16<F8>(v[2 * r]) || odd16<F8>(v[2 * r + 1])))
-                    odd |= 1u << (8 * s + 4 * h + r);
-                }
+                if (NA == 9) put(st + 8 * CH, r0 + 4 * h + (lane >> 3), lane & 7, pe[h]);
               }
-              store_pe();
             }
             fence_proxy_async();
           } else {
@@ -643,22 +670,40 @@ __global__ void __launch_bounds__(THREADS, 1) tree_mla_kernel(const __grid_const
         ml[0] = m_used;
         ml[1] = l;
       }
-      __nv_bfloat16* o = p.out + (size_t(c0) * p.H + r) * 512 + half * 256 + part * 128;
-      float* po = p.part_o + (size_t(max(it.part, 0)) * 128 + rank * 64 + row) * 512 + half * 256 + part * 128;
+      // O: a lane's row of 64 bf16 (32 fp32) columns at a time, transposed over four lanes, so that a store instruction
+      // writes eight whole 128-byte lines instead of a sector of 32 (2.3 us of a one-tile call's 3.5 us epilogue)
+      const int quad = (lane & 3) * 8, top = rank * 64 + (row & ~3);                // the four rows' first, in the tile
+      const int rows_left = n * p.H - it.row * 128 - top;
+      if (it.part < 0) {
+        __nv_bfloat16* o = p.out + (size_t(c0) * p.H + it.row * 128 + top) * 512 + half * 256 + part * 128 + 2 * quad;
 #pragma unroll 1
-      for (int c = 0; c < 128; c += 32) {
-        uint32_t v[32];
-        tmem_ld_32x32b_x32(t_lane + TM_O + part * 128 + c, v);
-        tmem_ld_wait();
-        if (it.part >= 0) {
-#pragma unroll
-          for (int k = 0; k < 32; k += 8) store32(po + c + k, v + k);
-        } else if (live) {
+        for (int c = 0; c < 128; c += 64) {
+          uint32_t v[32], x[32];
+          tmem_ld_32x32b_x32(t_lane + TM_O + part * 128 + c, x);
+          tmem_ld_wait();
 #pragma unroll
           for (int k = 0; k < 16; ++k)
-            v[k] = pack_bf16x2(__uint_as_float(v[2 * k]) * inv, __uint_as_float(v[2 * k + 1]) * inv);
-          store32(o + c, v);
-          store32(o + c + 16, v + 8);
+            v[k] = pack_bf16x2(__uint_as_float(x[2 * k]) * inv, __uint_as_float(x[2 * k + 1]) * inv);
+          tmem_ld_32x32b_x32(t_lane + TM_O + part * 128 + c + 32, x);
+          tmem_ld_wait();
+#pragma unroll
+          for (int k = 0; k < 16; ++k)
+            v[16 + k] = pack_bf16x2(__uint_as_float(x[2 * k]) * inv, __uint_as_float(x[2 * k + 1]) * inv);
+          quad_transpose(v, lane);
+#pragma unroll
+          for (int u = 0; u < 4; ++u)
+            if (u < rows_left) store32(o + u * 512 + c, v + 8 * u);
+        }
+      } else {
+        float* po = p.part_o + (size_t(it.part) * 128 + top) * 512 + half * 256 + part * 128 + quad;
+#pragma unroll 1
+        for (int c = 0; c < 128; c += 32) {
+          uint32_t v[32];
+          tmem_ld_32x32b_x32(t_lane + TM_O + part * 128 + c, v);
+          tmem_ld_wait();
+          quad_transpose(v, lane);
+#pragma unroll
+          for (int u = 0; u < 4; ++u) store32(po + u * 512 + c, v + 8 * u);
         }
       }
       tc_fence_before();
