@@ -37,7 +37,7 @@ cb::TreeLayout layout(const Tensor& cu, const Tensor& ctx, const Tensor& table, 
 // from L2.
 // -> int32 tensor (16-byte aligned parts): first [clusters + 1], items [*, 8], merges [*, 6], whole key tiles (request,
 // tile) [*, 2], first of them per request [B]; and the counts of CTA pairs, items, merges, partial results, whole key
-// tiles and key tiles over all items
+// tiles, key tiles over all items and the most partial results of a row tile
 std::tuple<Tensor, std::vector<int64_t>> tree_schedule(const std::vector<int64_t>& n, const std::vector<int64_t>& ctx,
                                                        int64_t H, int64_t clusters) {
   constexpr int64_t kTile = 128, kOver = 2, kPiece = 1;
@@ -130,7 +130,9 @@ std::tuple<Tensor, std::vector<int64_t>> tree_schedule(const std::vector<int64_t
       st[2 * k + 1] = int(t);
     }
   }
-  return {out, {used, n_items, int64_t(merges.size()), parts, n_stage, work}};
+  int64_t most = 0;
+  for (const auto& m : merges) most = std::max<int64_t>(most, m.n);
+  return {out, {used, n_items, int64_t(merges.size()), parts, n_stage, work, most}};
 }
 
 // work: tree_schedule's tensor on the device, counts its counts; buf: workspace of the partial outputs, then (m, l);
@@ -148,6 +150,7 @@ int tree_mla(const Tensor& q, const Tensor& kv, const Tensor& cu, const Tensor& 
   tw.merges = reinterpret_cast<const cb::TreeMerge*>(w + head + 8 * counts[1]);
   tw.clusters = int(counts[0]);
   tw.n_merges = int(counts[2]);
+  tw.most_parts = int(counts[6]);
   const int* st = w + head + 8 * counts[1] + 6 * counts[2];
   tw.stage = reinterpret_cast<const int2*>(st);
   tw.stage_at = st + 2 * counts[4];

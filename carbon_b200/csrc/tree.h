@@ -27,7 +27,7 @@ struct TreeWork {
   const int* first;        // [clusters + 1]
   const TreeItem* items;
   const TreeMerge* merges;
-  int clusters, n_merges;
+  int clusters, n_merges, most_parts;     // most_parts: of one row tile
   // 128-row blocks of the staging buffer, one per whole key tile before the tree: (request, key tile), and each
   // request's first block
   const int2* stage;

@@ -720,29 +720,31 @@ __global__ void __launch_bounds__(THREADS, 1) tree_mla_kernel(const __grid_const
 }
 
 // out = sum_s 2^(m_s - M) O_s / (sum_s 2^(m_s - M) l_s + sink): one CTA per row of a split row tile, four of the 512
-// dims per thread; eight partial rows are in flight, with a running maximum.
-__global__ void __launch_bounds__(128) tree_merge_kernel(const TreeMerge* __restrict__ merges, int H,
-                                                         const float* __restrict__ part_o,
-                                                         const float* __restrict__ part_ml,
-                                                         const float* __restrict__ sink,
-                                                         __nv_bfloat16* __restrict__ out) {
+// dims per thread, eight partial rows in flight with a running maximum.  With more than eight partial rows G groups of
+// threads take every G-th one and are joined through shared memory.
+template <int G>
+__global__ void __launch_bounds__(128 * G) tree_merge_kernel(const TreeMerge* __restrict__ merges, int H,
+                                                             const float* __restrict__ part_o,
+                                                             const float* __restrict__ part_ml,
+                                                             const float* __restrict__ sink,
+                                                             __nv_bfloat16* __restrict__ out) {
   const TreeMerge mg = merges[blockIdx.x];              // made by the host
   pdl_entry();
-  const int row = blockIdx.y, r = mg.row * 128 + row;
+  const int row = blockIdx.y, r = mg.row * 128 + row, group = threadIdx.x >> 7, dim = threadIdx.x & 127;
   if (r >= mg.rows) return;
   const float2* ml = reinterpret_cast<const float2*>(part_ml) + size_t(mg.part) * 128 + row;
-  const float4* po = reinterpret_cast<const float4*>(part_o) + (size_t(mg.part) * 128 + row) * 128 + threadIdx.x;
+  const float4* po = reinterpret_cast<const float4*>(part_o) + (size_t(mg.part) * 128 + row) * 128 + dim;
   float M = sink ? sink[r % H] * 1.4426950408889634f : -INFINITY;
-  float L = sink ? 1.f : 0.f;
+  float L = sink && group == 0 ? 1.f : 0.f;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int s0 = 0; s0 < mg.n; s0 += 8) {
+  for (int s0 = group; s0 < mg.n; s0 += 8 * G) {
     float2 v[8];
     float4 o[8];
 #pragma unroll
     for (int s = 0; s < 8; ++s) {
-      const bool in = s0 + s < mg.n;
-      v[s] = in ? ml[(s0 + s) * 128] : make_float2(-INFINITY, 0.f);
-      o[s] = in ? po[size_t(s0 + s) * 128 * 128] : make_float4(0.f, 0.f, 0.f, 0.f);
+      const int at = s0 + s * G;
+      v[s] = at < mg.n ? ml[at * 128] : make_float2(-INFINITY, 0.f);
+      o[s] = at < mg.n ? po[size_t(at) * 128 * 128] : make_float4(0.f, 0.f, 0.f, 0.f);
     }
     float top = M;
 #pragma unroll
@@ -758,8 +760,30 @@ __global__ void __launch_bounds__(128) tree_merge_kernel(const TreeMerge* __rest
       acc.x += w * o[s].x; acc.y += w * o[s].y; acc.z += w * o[s].z; acc.w += w * o[s].w;
     }
   }
+  if constexpr (G > 1) {
+    __shared__ float4 s_acc[G][128];
+    __shared__ float2 s_ml[G];
+    s_acc[group][dim] = acc;
+    if (dim == 0) s_ml[group] = make_float2(M, L);
+    __syncthreads();
+    if (group) return;
+    float top = M;
+#pragma unroll
+    for (int k = 1; k < G; ++k) top = fmaxf(top, s_ml[k].x);
+    const float ref = top == -INFINITY ? 0.f : top;
+    const float keep = exp2f(M - ref);
+    acc.x *= keep; acc.y *= keep; acc.z *= keep; acc.w *= keep;
+    L *= keep;
+#pragma unroll
+    for (int k = 1; k < G; ++k) {
+      const float w = exp2f(s_ml[k].x - ref);
+      const float4 o = s_acc[k][dim];
+      L += w * s_ml[k].y;
+      acc.x += w * o.x; acc.y += w * o.y; acc.z += w * o.z; acc.w += w * o.w;
+    }
+  }
   const float inv = L == 0.f ? 0.f : 1.f / L;
-  reinterpret_cast<uint2*>(out + (size_t(mg.c0) * H + r) * 512)[threadIdx.x] =
+  reinterpret_cast<uint2*>(out + (size_t(mg.c0) * H + r) * 512)[dim] =
       make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
 }
 
@@ -847,8 +871,9 @@ cudaError_t tree_mla(const void* q, int T, int H, int D, bool f8, const void* kv
   cudaLaunchAttribute attr[2];
   const cudaLaunchConfig_t cfg = pair_config(work.clusters, attr, s);
   if ((e = cudaLaunchKernelEx(&cfg, f, m, p)) != cudaSuccess || !work.n_merges) return e;
-  return launch_k(tree_merge_kernel, dim3(work.n_merges, 128), 128, 0, s, work.merges, H, part_o, part_ml, sink,
-                  p.out);
+  const bool many = work.most_parts > 8;
+  return launch_k(many ? tree_merge_kernel<4> : tree_merge_kernel<1>, dim3(work.n_merges, 128), many ? 512 : 128, 0, s,
+                  work.merges, H, part_o, part_ml, sink, p.out);
 }
 
 }  // namespace cb

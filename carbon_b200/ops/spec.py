@@ -185,7 +185,7 @@ def tree_mla(q: torch.Tensor, kv: torch.Tensor, plan: TreePlan, scale: float, d_
             _need("tree_mla: sink", sink, dev, torch.float32)
         out = torch.empty(T, H, 512, dtype=torch.bfloat16, device=q.device)
         if T:
-            parts, tiles, work = plan._counts[3:]
+            parts, tiles, work = plan._counts[3:6]
             # Whole key tiles that TMA cannot take from the cache as they lie (fp8 rows, small pages) are fed by the
             # kernel's warps (4.0 us a tile and CTA pair), or expanded to dense rows first (2.0 us a tile then, and
             # 2.8 us of every pair's time per staged tile; a launch): worth it from two row tiles per key tile and a
