@@ -336,26 +336,53 @@ __global__ void __launch_bounds__(kThreads, 2) tree_verify_kernel(
   }
 }
 
-// One CTA per (cache, request); a thread owns 16 (or 4) bytes of the row and walks the path.  Node path[k] >= k and the
-// path ascends, so a slot is written only after every read of it: per thread the order k = 1, 2, ... is enough.
+// One CTA per (cache, request); a thread owns 16 (or 4) bytes of the row and walks the path, eight rows in flight.  Node
+// path[k] >= k and the path ascends, so a slot is written only after every read of it: per thread the order of k is
+// enough, and reading a later row early is harmless.  The rows' slots are looked up once per CTA, in parallel.
 template <typename V>
-__global__ void tree_commit_kernel(const int64_t* __restrict__ caches, TreeLayout lay, int N,
-                                   const int* __restrict__ path, const int* __restrict__ n_accepted) {
-  pdl_entry();
+__global__ void __launch_bounds__(256) tree_commit_kernel(const int64_t* __restrict__ caches, TreeLayout lay, int N,
+                                                          const int* __restrict__ path,
+                                                          const int* __restrict__ n_accepted) {
+  __shared__ int s_from[kNodes], s_to[kNodes];
+  __shared__ int s_moves;
   const int b = blockIdx.y;
-  const int n = lay.cu[b + 1] - lay.cu[b], c = lay.ctx[b];
-  const int m = min(n_accepted[b], n - 1);
+  const int n = lay.cu[b + 1] - lay.cu[b], c = lay.ctx[b];               // made by the host
   char* base = reinterpret_cast<char*>(caches[2 * blockIdx.x]);
   const int64_t bytes = caches[2 * blockIdx.x + 1];
-  auto at = [&](int i) {
-    const int p = c + i;
-    return base + (int64_t(lay.table[size_t(b) * lay.P + p / lay.page]) * lay.page + p % lay.page) * bytes;
-  };
+  pdl_entry();
+  const int m = min(n_accepted[b], n - 1);
+  if (m <= 0) return;
+  if (threadIdx.x < 32) {
+    auto slot = [&](int i) {
+      const int p = c + i;
+      return lay.table[size_t(b) * lay.P + p / lay.page] * lay.page + p % lay.page;
+    };
+    int moves = 0;
+    for (int k0 = 1; k0 <= m; k0 += 32) {
+      const int k = k0 + int(threadIdx.x);
+      const int i = k <= m ? path[b * N + k] : -1;
+      const bool move = i > k && i < n;                // else already in place, or not a node
+      const uint32_t all = __ballot_sync(~0u, move);
+      if (move) {
+        const int at = moves + __popc(all & ((1u << threadIdx.x) - 1));
+        s_from[at] = slot(i);
+        s_to[at] = slot(k);
+      }
+      moves += __popc(all);
+    }
+    if (threadIdx.x == 0) s_moves = moves;
+  }
+  __syncthreads();
+  const int moves = s_moves;
   for (int64_t o = threadIdx.x * int64_t(sizeof(V)); o < bytes; o += blockDim.x * int64_t(sizeof(V)))
-    for (int k = 1; k <= m; ++k) {
-      const int i = path[b * N + k];
-      if (i <= k || i >= n) continue;       // already in place, or not a node
-      *reinterpret_cast<V*>(at(k) + o) = *reinterpret_cast<const V*>(at(i) + o);
+    for (int k0 = 0; k0 < moves; k0 += 8) {
+      V v[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (k0 + k < moves) v[k] = *reinterpret_cast<const V*>(base + s_from[k0 + k] * bytes + o);
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (k0 + k < moves) *reinterpret_cast<V*>(base + s_to[k0 + k] * bytes + o) = v[k];
     }
 }
 
