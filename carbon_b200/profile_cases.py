@@ -1,6 +1,6 @@
 """Small, self-contained kernel cases for profiler captures (one launch of one kernel each, a few GB at most).
 
-    python -m carbon_b200.profile_cases gemm|grouped|moe_decode|attn|decode|decode_fp8|boundary|indexer|indexer_decode|ep_moe|oproj_a2a
+    python -m carbon_b200.profile_cases gemm|grouped|moe_decode|attn|decode|decode_fp8|boundary|indexer|indexer_decode|ep_moe|oproj_a2a|tree|tree_verify
 
 Each case sets up inputs larger than L2 where it can, runs its kernel twice (warm-up + the launch to capture) and
 exits 0, so that ``ncu -k regex:<kernel> -s 1 -c 1`` captures exactly one warm launch.
@@ -189,9 +189,48 @@ def oproj_a2a():
         f.heads_to_tokens(o)
 
 
+def _trees(requests, nodes, ctx, heads=128):
+    """A plan of equal requests with two-way branching trees (node i's parent is (i - 1) // 2) on consecutive pages."""
+    from .ops.spec import TreePlan
+
+    parents = [[-1] + [(i - 1) // 2 for i in range(1, nodes)]] * requests
+    need = -(-(ctx + nodes) // 64)
+    tables = [list(range(1 + b * need, 1 + (b + 1) * need)) for b in range(requests)]
+    return TreePlan(tables, [ctx] * requests, parents, 64, n_heads=heads), (1 + requests * need) * 64
+
+
+def tree():
+    """Tree attention: 12 requests of 5,000 cached keys (bf16 rows), trees of 24 nodes, 128 heads."""
+    from .ops.spec import tree_mla
+
+    plan, slots = _trees(12, 24, 5000)
+    kv = torch.randn(slots, 576, device="cuda").to(torch.bfloat16)
+    q = torch.randn(plan.T, 128, 576, device="cuda").to(torch.bfloat16)
+    for _ in range(2):
+        tree_mla(q, kv, plan, 192 ** -0.5)
+    plan.check()
+
+
+def tree_verify():
+    """Tree verification: 32 requests, trees of 12 nodes drawn from a draft model's distributions, vocabulary 129,280."""
+    from .ops.spec import tree_verify as verify
+
+    plan, _ = _trees(32, 12, 0)
+    V = 129280
+    base = torch.randn(plan.T, V, device="cuda") * 5
+    logits = base + 0.5 * torch.randn(plan.T, V, device="cuda")
+    draft = torch.softmax(base + 0.5 * torch.randn(plan.T, V, device="cuda"), -1)
+    up = torch.tensor([12 * b + max(0, (i - 1) // 2) for b in range(32) for i in range(12)], device="cuda")
+    tokens = torch.multinomial(draft[up], 1)[:, 0].int()
+    u, e = torch.rand(plan.T, device="cuda"), torch.empty(32, V, device="cuda").exponential_()
+    for _ in range(2):
+        verify(logits, tokens, plan, u, e, torch.full((32,), 0.8, device="cuda"), draft)
+
+
 if __name__ == "__main__":
     {"gemm": gemm, "grouped": grouped, "moe_decode": moe_decode, "attn": attn, "decode": decode,
      "decode_fp8": decode_fp8, "boundary": boundary,
-     "indexer": indexer, "indexer_decode": indexer_decode, "ep_moe": ep_moe, "oproj_a2a": oproj_a2a}[sys.argv[1]]()
+     "indexer": indexer, "indexer_decode": indexer_decode, "ep_moe": ep_moe, "oproj_a2a": oproj_a2a,
+     "tree": tree, "tree_verify": tree_verify}[sys.argv[1]]()
     torch.cuda.synchronize()
     print("ok", sys.argv[1])
