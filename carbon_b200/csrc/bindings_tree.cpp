@@ -2,6 +2,7 @@
 // arguments' checks, outputs and workspaces belong to carbon_b200/ops/spec.py, which raises Python exceptions (a C++
 // exception is not safe in a build whose libstdc++ is linked statically beside torch's shared one).
 #include <torch/extension.h>
+#include <torch/cuda.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <algorithm>
@@ -135,6 +136,66 @@ std::tuple<Tensor, std::vector<int64_t>> tree_schedule(const std::vector<int64_t
   return {out, {used, n_items, int64_t(merges.size()), parts, n_stage, work, most}};
 }
 
+// The lists of a TreePlan with the default masks (each node's ancestors and itself), in one pinned int32 buffer:
+// work (tree_schedule) | masks [T, 2] | cu [B + 1] | ctx [B] | req [T] | parent [T] | pos [T] | slot [T] | table [B, P] |
+// status (0).  Returns (0, buffer, counts, [work length, T, N, P, largest page]), or (-1, ...) where an argument does not
+// fit: the caller's own checks then say which.
+std::tuple<int, Tensor, std::vector<int64_t>, std::vector<int64_t>> tree_plan(
+    const std::vector<std::vector<int64_t>>& tables, const std::vector<int64_t>& ctx,
+    const std::vector<std::vector<int64_t>>& parents, int64_t page, int64_t H, int64_t clusters) {
+  const int64_t B = int64_t(parents.size());
+  const auto refuse = std::make_tuple(-1, Tensor(), std::vector<int64_t>(), std::vector<int64_t>());
+  if (int64_t(tables.size()) != B || int64_t(ctx.size()) != B || page < 1 || H < 1) return refuse;
+  std::vector<int64_t> n(B);
+  int64_t T = 0, N = 0, P = 1, top = -1;
+  for (int64_t b = 0; b < B; ++b) {
+    const int64_t k = n[b] = int64_t(parents[b].size()), have = int64_t(tables[b].size());
+    if (k > 64 || ctx[b] < 0 || (ctx[b] + k + page - 1) / page > have) return refuse;
+    for (int64_t i = 0; i < k; ++i)
+      if (i ? parents[b][i] < 0 || parents[b][i] >= i : parents[b][i] != -1) return refuse;
+    for (int64_t pg : tables[b]) {
+      if (pg < 0 || (pg + 1) * page > (int64_t(1) << 31) - 1) return refuse;
+      top = std::max(top, pg);
+    }
+    T += k;
+    N = std::max(N, k);
+    P = std::max(P, have);
+  }
+  Tensor work = torch::empty({0}, torch::kInt32);
+  std::vector<int64_t> counts;
+  if (T) std::tie(work, counts) = tree_schedule(n, ctx, H, clusters);
+  const int64_t W = work.numel();
+  auto out = torch::empty({W + 2 * T + B + 1 + B + 4 * T + B * P + 1},
+                          torch::TensorOptions().dtype(torch::kInt32).pinned_memory(torch::cuda::is_available()));
+  int* o = ptr<int>(out);
+  if (W) std::memcpy(o, ptr<int>(work), W * sizeof(int));
+  int* masks = o + W;
+  int* cu = masks + 2 * T;
+  int* cx = cu + B + 1;
+  int *req = cx + B, *par = req + T, *pos = par + T, *slot = pos + T, *table = slot + T;
+  int64_t t = 0;
+  cu[0] = 0;
+  for (int64_t b = 0; b < B; ++b) {
+    uint64_t mask[64];
+    int depth[64];
+    for (int64_t i = 0; i < n[b]; ++i, ++t) {
+      const int64_t up = parents[b][i], at = ctx[b] + i;
+      mask[i] = (uint64_t(1) << i) | (i ? mask[up] : 0);
+      depth[i] = i ? depth[up] + 1 : 0;
+      std::memcpy(masks + 2 * t, &mask[i], 8);
+      req[t] = int(b);
+      par[t] = int(up);
+      pos[t] = int(ctx[b] + depth[i]);
+      slot[t] = int(tables[b][at / page] * page + at % page);
+    }
+    cu[b + 1] = int(t);
+    cx[b] = int(ctx[b]);
+    for (int64_t i = 0; i < P; ++i) table[b * P + i] = i < int64_t(tables[b].size()) ? int(tables[b][i]) : 0;
+  }
+  table[B * P] = 0;
+  return {0, out, counts, {W, T, N, P, top}};
+}
+
 // work: tree_schedule's tensor on the device, counts its counts; buf: workspace of the partial outputs, then (m, l);
 // staged: workspace of the dense key rows, if they are to be staged
 int tree_mla(const Tensor& q, const Tensor& kv, const Tensor& cu, const Tensor& ctx, const Tensor& table,
@@ -204,7 +265,7 @@ int tree_commit(const Tensor& caches, int64_t max_row, bool wide, const Tensor& 
 }  // namespace
 
 void register_tree(pybind11::module_& m) {
-  m.def("tree_schedule", &tree_schedule);
+  m.def("tree_plan", &tree_plan);
   m.def("tree_mla_clusters", [] { return cb::tree_mla_clusters(); });
   m.def("tree_mla", &tree_mla);
   m.def("tree_verify", &tree_verify);

@@ -579,7 +579,7 @@ class Engine:
         listed = cfg.use_indexer or cfg.engram_layers or cfg.attn_kind == "latent_mqa"
         key_slots = self._tree_key_slots(plan) if listed else torch.zeros(plan.T, 1, dtype=torch.int32)
         late = torch.tensor([r.late_from for r, k in zip(reqs, plan.n) for _ in range(k)], dtype=torch.int32)
-        fb = ForwardBatch(ids=ids, pos=plan.pos, out_loc=torch.tensor(plan.node_slots(), dtype=torch.int32).to(dev),
+        fb = ForwardBatch(ids=ids, pos=plan.pos, out_loc=plan.slot,
                           is_prefill=False, key_slots=key_slots.to(dev), n_keys=plan.pos + 1, late_from=late.to(dev),
                           tree=plan)
         with self.metrics.step("verify", plan.T, len(reqs)):
@@ -610,18 +610,18 @@ class Engine:
     @staticmethod
     def _tree_key_slots(plan) -> torch.Tensor:
         """[T, longest] int32: the cache slots of each node's keys in order (context, then its branch), -1 padded."""
-        ps = plan.page_size
-        width = max(p + 1 for p in plan.pos_list)
+        ps, pos, cu = plan.page_size, plan.pos_list, plan.cu_list
+        width = max(p + 1 for p in pos)
         out = torch.full((plan.T, width), -1, dtype=torch.int32)
         for b in range(plan.B):
-            c, lo = plan.ctx_list[b], plan.cu_list[b]
+            c, lo = plan.ctx_list[b], cu[b]
             tab = torch.tensor(plan.tables_list[b], dtype=torch.int32)
             slots = (tab[:, None] * ps + torch.arange(ps, dtype=torch.int32)).flatten()
             out[lo:lo + plan.n[b], :c] = slots[:c]
             for i, par in enumerate(plan.parents_list[b]):
                 if par >= 0:
-                    out[lo + i, c:plan.pos_list[lo + i]] = out[lo + par, c:plan.pos_list[lo + i]]
-                out[lo + i, plan.pos_list[lo + i]] = slots[c + i]
+                    out[lo + i, c:pos[lo + i]] = out[lo + par, c:pos[lo + i]]
+                out[lo + i, pos[lo + i]] = slots[c + i]
         return out
 
     def generate_speculative(self, prompts: List[Sequence[int]], max_new_tokens: int, drafter=None, n_draft: int = 5,

@@ -51,18 +51,44 @@ class TreePlan:
 
     def __init__(self, page_tables: Sequence[Sequence[int]], ctx: Sequence[int], parents: Sequence[Sequence[int]],
                  page_size: int, n_heads: int = 1, device="cuda", masks: Optional[Sequence[Sequence[int]]] = None):
+        self.device = torch.device(device)
+        cuda = self.device.type == "cuda"
+        if cuda and self.device.index is None:
+            self.device = torch.device("cuda", torch.cuda.current_device())
+        self.page_size, self.n_heads = int(page_size), int(n_heads)
+        self.ctx_list, self.tables_list, self.parents_list = list(ctx), page_tables, parents
+        code = -1
+        if cuda and masks is None:
+            code, host, self._counts, meta = ext().tree_plan(page_tables, self.ctx_list, parents, self.page_size,
+                                                             self.n_heads, _clusters(self.device))
+        if code:                            # other devices, given masks, and arguments that do not fit (raises)
+            host, meta = self._lists(masks)
+        w, T, self.N, P, self.max_page = meta
+        self.n = [len(p) for p in parents]
+        B = self.B = len(self.n)
+        self.T = T
+        self._host = host
+        dev = host.to(self.device, non_blocking=True)
+        self._work = dev[:w]
+        self.mask = dev[w:w + 2 * T].view(torch.int64)
+        self.status = dev[-1:]              # error code of a device-side wait that ran out (0: none)
+        at = self._at = w + 2 * T
+        out = []
+        for k in (B + 1, B, T, T, T, T, B * P):
+            out.append(dev[at:at + k])
+            at += k
+        self.cu, self.ctx, self.req, self.parent, self.pos, self.slot, self.table = out
+        self.table = self.table.view(B, P)
+
+    def _lists(self, masks):
+        """The plan's lists in one buffer, as the native builder lays them out: (buffer, lengths)."""
+        page_tables, ctx, parents, page_size = self.tables_list, self.ctx_list, self.parents_list, self.page_size
         B = len(parents)
         if len(page_tables) != B or len(ctx) != B or (masks is not None and len(masks) != B):
             raise ValueError("TreePlan: page_tables, ctx, parents (and masks) need one entry per request")
-        if page_size < 1 or n_heads < 1:
+        if page_size < 1 or self.n_heads < 1:
             raise ValueError("TreePlan: page_size and n_heads must be positive")
-        self.n = [len(p) for p in parents]
-        self.device = torch.device(device)
-        if self.device.type == "cuda" and self.device.index is None:
-            self.device = torch.device("cuda", torch.cuda.current_device())
-        self.page_size, self.n_heads = int(page_size), int(n_heads)
-        self.B, self.T, self.N = B, sum(self.n), max(self.n, default=0)
-        cu, req, par, pos, bits = [0], [], [], [], []
+        cu, req, par, pos, slot, bits = [0], [], [], [], [], []
         for b, (p, c, tab) in enumerate(zip(parents, ctx, page_tables)):
             k = len(p)
             if k > MAX_NODES:
@@ -72,6 +98,8 @@ class TreePlan:
                                  f"and nodes need {c + k}")
             if any(pg < 0 for pg in tab):
                 raise ValueError(f"TreePlan: request {b} has a negative page")
+            if any((pg + 1) * page_size > 2 ** 31 - 1 for pg in tab):
+                raise ValueError(f"TreePlan: request {b} has a page past 2^31 slots")
             depth = []
             for i, q in enumerate(p):
                 if not (q == -1 if i == 0 else 0 <= q < i):
@@ -86,37 +114,33 @@ class TreePlan:
             req += [b] * k
             par += p
             pos += [c + d for d in depth]
-        self.ctx_list, self.tables_list, self.parents_list = [int(c) for c in ctx], page_tables, parents
-        self.cu_list, self.pos_list = cu, pos
-        self.max_page = max((pg for tab in page_tables for pg in tab), default=-1)
+            slot += [tab[(c + i) // page_size] * page_size + (c + i) % page_size for i in range(k)]
         P = max([len(t) for t in page_tables] + [1])
         flat = []
         for tab in page_tables:
             flat += list(tab)
             flat += [0] * (P - len(tab))
-        # one host buffer, one copy: the attention's work (16-byte aligned parts), masks (64 bits), the 32-bit lists
-        T = self.T
-        words = torch.tensor(bits, dtype=torch.int64).view(torch.int32)
         work, self._counts = torch.zeros(0, dtype=torch.int32), []
-        if self.device.type == "cuda" and T:
-            work, self._counts = ext().tree_schedule(self.n, [int(c) for c in ctx], self.n_heads,
-                                                     _clusters(self.device))
-        ints = torch.tensor(cu + list(ctx) + req + par + pos + flat + [0], dtype=torch.int32)
-        host = torch.cat([work, words, ints])
-        if self.device.type == "cuda":
-            host = host.pin_memory()
-        dev = host.to(self.device, non_blocking=True)
-        w = work.numel()                    # a multiple of 4
-        self._work = dev[:w]
-        self.mask = dev[w:w + 2 * T].view(torch.int64)
-        self.status = dev[-1:]              # error code of a device-side wait that ran out (0: none)
-        at = w + 2 * T
-        out = []
-        for k in (B + 1, B, T, T, T, B * P):
-            out.append(dev[at:at + k])
-            at += k
-        self.cu, self.ctx, self.req, self.parent, self.pos, self.table = out
-        self.table = self.table.view(B, P)
+        cuda = self.device.type == "cuda"
+        if cuda and cu[-1]:
+            got = ext().tree_plan(page_tables, ctx, parents, page_size, self.n_heads, _clusters(self.device))
+            work, self._counts = got[1][:got[3][0]], got[2]
+        host = torch.cat([work, torch.tensor(bits, dtype=torch.int64).view(torch.int32),
+                          torch.tensor(cu + list(ctx) + req + par + pos + slot + flat + [0], dtype=torch.int32)])
+        top = max((pg for tab in page_tables for pg in tab), default=-1)
+        return (host.pin_memory() if cuda else host), (work.numel(), cu[-1], max((len(p) for p in parents), default=0),
+                                                       P, top)
+
+    @property
+    def cu_list(self) -> List[int]:
+        """First node row of each request, and the number of rows."""
+        return self._host[self._at:self._at + self.B + 1].tolist()
+
+    @property
+    def pos_list(self) -> List[int]:
+        """Position of each node in its sequence (its depth behind the context)."""
+        at = self._at + 2 * self.B + 1 + 2 * self.T
+        return self._host[at:at + self.T].tolist()
 
     def check(self) -> None:
         """Raise if a kernel of this plan gave up a wait (reads from the device)."""
@@ -130,10 +154,9 @@ class TreePlan:
         return [tab[i // ps] * ps + i % ps for i in range(n)]
 
     def node_slots(self) -> List[int]:
-        """Cache slot of every node row."""
-        ps = self.page_size
-        return [tab[(c + i) // ps] * ps + (c + i) % ps
-                for tab, c, k in zip(self.tables_list, self.ctx_list, self.n) for i in range(k)]
+        """Cache slot of every node row (``slot`` on the device)."""
+        at = self._at + 2 * self.B + 1 + 3 * self.T
+        return self._host[at:at + self.T].tolist()
 
     def _check(self, what: str, slots: int):
         if (self.max_page + 1) * self.page_size > slots:
@@ -200,8 +223,9 @@ def tree_mla(q: torch.Tensor, kv: torch.Tensor, plan: TreePlan, scale: float, d_
         return out
     out = torch.zeros(T, H, d_latent)
     mla = D > d_latent
+    cu = plan.cu_list
     for b in range(plan.B):
-        lo, hi = plan.cu_list[b], plan.cu_list[b + 1]
+        lo, hi = cu[b], cu[b + 1]
         rows = kv[torch.tensor(plan.slots(b), dtype=torch.long)]
         rows = R.dequant_latent_fp8(rows, d_latent, D - d_latent if mla else 0, mla) if f8 else rows.float()
         out[lo:hi] = R.tree_attention(q[lo:hi].float(), rows, plan.ctx_list[b], plan.mask[lo:hi].tolist(), scale,
@@ -264,8 +288,9 @@ def tree_verify(logits: torch.Tensor, tokens: torch.Tensor, plan: TreePlan, unif
     _check_verify(logits, tokens, plan, uniforms, noise, temperature, draft_probs)
     v = TreeVerdict(torch.full((B, N), -1, dtype=torch.int32), torch.full((B,), -1, dtype=torch.int32),
                     torch.full((B, N), -1, dtype=torch.int32), torch.zeros(B, N))
+    cu = plan.cu_list
     for b in range(B):
-        lo, hi = plan.cu_list[b], plan.cu_list[b + 1]
+        lo, hi = cu[b], cu[b + 1]
         if lo == hi:
             continue
         path, toks, lps = R.tree_verify(logits[lo:hi].float(), tokens[lo:hi], plan.parents_list[b], uniforms[lo:hi],

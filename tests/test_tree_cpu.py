@@ -180,3 +180,67 @@ def test_cache_rows_refusals():
         spec.CacheRows([torch.zeros(8, 4)[:, :2]])
     with pytest.raises(ValueError, match="4 bytes"):
         spec.CacheRows([torch.zeros(8, 3, dtype=torch.uint8)])
+
+
+def test_native_plan_is_the_same():
+    """The native builder's buffer behind the attention's work equals the Python lists; it refuses what they refuse."""
+    from carbon_b200.ops._ext import available, ext
+
+    if not available():
+        pytest.skip("the extension is not built")
+    parents = [[-1, 0, 0, 1, 3], [], [-1] + list(range(63)), [-1]]
+    ctx, page = [5, 2, 130, 0], 7
+    tables = [[3, 9], [4], list(range(20, 48)), [0, 77]]
+    plan = spec.TreePlan(tables, ctx, parents, page, n_heads=16, device="cpu")
+    code, host, counts, meta = ext().tree_plan(tables, ctx, parents, page, 16, 74)
+    assert code == 0 and meta[1:] == [70, 64, 28, 77] and len(counts) == 7
+    assert torch.equal(host[meta[0]:], plan._host)
+    assert plan.node_slots() == [plan.slots(b)[ctx[b] + i] for b in range(4) for i in range(plan.n[b])]
+    for bad in (dict(parents=[[-1, 1]] + parents[1:]), dict(ctx=[10, 2, 130, 0]), dict(ctx=[-1, 2, 130, 0]),
+                dict(parents=[[-1] + [0] * 64] + parents[1:]), dict(tables=[[3, -9]] + tables[1:]), dict(ctx=[5]),
+                dict(tables=[[3, 2 ** 31 // 7]] + tables[1:])):
+        a = dict(tables=tables, ctx=ctx, parents=parents)
+        a.update(bad)
+        assert ext().tree_plan(a["tables"], a["ctx"], a["parents"], page, 16, 74)[0] == -1
+        with pytest.raises(ValueError):
+            spec.TreePlan(a["tables"], a["ctx"], a["parents"], page, n_heads=16, device="cpu")
+
+
+@pytest.mark.parametrize("clusters,heads", [(74, 128), (74, 5), (1, 16), (7, 64)])
+def test_schedule_covers_every_key_tile_once(clusters, heads):
+    from carbon_b200.ops._ext import available, ext
+
+    if not available():
+        pytest.skip("the extension is not built")
+    n = [1, 0, 6, 64, 17, 1]
+    ctx = [0, 300, 127, 128, 9001, 4000]
+    parents = [[-1] + [0] * (k - 1) if k else [] for k in n]
+    tables = [list(range((c + k) // 64 + 1)) for c, k in zip(ctx, n)]
+    _, host, (used, items, merges, parts, whole, work, most), meta = ext().tree_plan(tables, ctx, parents, 64, heads,
+                                                                                     clusters)
+    w = host[:meta[0]].tolist()
+    first, head = w[:used + 1], (used + 4) // 4 * 4
+    it = [w[head + 8 * i:head + 8 * i + 8] for i in range(items)]
+    mg = [w[head + 8 * items + 6 * i:head + 8 * items + 6 * i + 6] for i in range(merges)]
+    assert used <= clusters and first[0] == 0 and first[-1] == items and all(a < b for a, b in zip(first, first[1:]))
+    cu = [sum(n[:b]) for b in range(len(n))]
+    rows = {}
+    for b, row, tile, tiles, part, c, c0, k in it:
+        assert (c, c0, k) == (ctx[b], cu[b], n[b]) and tiles > 0
+        rows.setdefault((b, row), []).append((tile, tiles, part))
+    assert set(rows) == {(b, r) for b, k in enumerate(n) for r in range((k * heads + 127) // 128)}
+    for (b, row), pieces in rows.items():
+        at = 0
+        for tile, tiles, _ in sorted(pieces):
+            assert tile == at
+            at += tiles
+        assert at == (ctx[b] + n[b] + 127) // 128
+        ids = sorted(p for _, _, p in pieces)
+        if len(pieces) == 1:
+            assert ids == [-1]
+        else:
+            assert [row, ids[0], len(ids), cu[b], n[b] * heads, 0] in mg and ids == list(range(ids[0], ids[0] + len(ids)))
+    assert work == sum(x[3] for x in it) and parts == sum(m[2] for m in mg) and most == max([m[2] for m in mg] + [0])
+    at = head + 8 * items + 6 * merges
+    want = [(b, t) for b in range(len(n)) for t in range(ctx[b] // 128) if n[b]]
+    assert whole == len(want) and [tuple(w[at + 2 * i:at + 2 * i + 2]) for i in range(whole)] == want
