@@ -316,14 +316,16 @@ class CacheRows:
         self.slots = min(c.shape[0] for c in self.caches)
         rows = []
         for c in self.caches:
-            nbytes = c[0].numel() * c.element_size() if c.shape[0] else 0
+            nbytes = c.numel() // max(1, c.shape[0]) * c.element_size()
             if c.device != first.device or not c.is_contiguous() or nbytes % 4 or not nbytes:
                 raise ValueError("CacheRows: caches must be contiguous, on one device and have rows of a multiple of "
                                  "4 bytes")
             rows += [c.data_ptr(), nbytes]
         self.max_row = max(rows[1::2])
         self.wide = all(x % 16 == 0 for x in rows)
-        self.table = torch.tensor(rows, dtype=torch.int64).view(-1, 2).to(first.device)
+        table = torch.tensor(rows, dtype=torch.int64).view(-1, 2)
+        self._host = table.pin_memory() if first.is_cuda else table
+        self.table = self._host.to(first.device, non_blocking=True)
 
 
 def tree_commit(rows: CacheRows, plan: TreePlan, path: torch.Tensor, n_accepted: torch.Tensor) -> None:
