@@ -467,18 +467,19 @@ __global__ void __launch_bounds__(THREADS, 1) tree_mla_kernel(const __grid_const
             } else {
               uint4 pe[2];
 #pragma unroll
-              for (int h = 0; h < 2; ++h) {             // four rows at a time
+              for (int h = 0; h < 2; ++h) {             // four rows at a time; rows past the end are not read
                 uint4 v[8];
 #pragma unroll
-                for (int r = 0; r < 4; ++r)
-#pragma unroll
-                  for (int k = 0; k < 2; ++k) v[2 * r + k] = reinterpret_cast<const uint4*>(at(now, 8 * u + 4 * h + r))[k * 32 + lane];
+                for (int r = 0; r < 4; ++r) {
+                  const uint4* src = reinterpret_cast<const uint4*>(at(now, 8 * u + 4 * h + r));
+                  v[2 * r] = v[2 * r + 1] = zero;
+                  if (4 * h + r < rows) { v[2 * r] = src[lane]; v[2 * r + 1] = src[32 + lane]; }
+                }
                 if (NA == 9) pe[h] = reinterpret_cast<const uint4*>(at(now, 8 * u + 4 * h + (lane >> 3)))[64 + (lane & 7)];
                 if (h == 0) ok = wait(&pv0[s], ph ^ 1, kErrTimeoutEmpty) && wait(&pv1[s], ph ^ 1, kErrTimeoutEmpty);
                 if (tail) {
 #pragma unroll
                   for (int r = 0; r < 4; ++r) {
-                    if (4 * h + r >= rows) v[2 * r] = v[2 * r + 1] = zero;
                     if (__any_sync(~0u, odd16<F8>(v[2 * r]) || odd16<F8>(v[2 * r + 1]))) odd |= 1u << (8 * s + 4 * h + r);
                   }
                   if (NA == 9) {
