@@ -7,10 +7,13 @@
 #include "ptx.cuh"
 #include "tree.h"
 
+#include <algorithm>
+#include <atomic>
+
 namespace cb {
 namespace tree {
 
-constexpr int kNodes = 64, kThreads = 512, kUnroll = 8, kWide = 16, kMaxCluster = 16;
+constexpr int kNodes = 64, kThreads = 512, kUnroll = 8, kWide = 16, kMaxCluster = 16, kShare = 1024;
 constexpr float kLog2e = 1.4426950408889634f;
 
 CB_DEVICE float ex2v(float x) {
@@ -25,10 +28,11 @@ CB_DEVICE float ex2v(float x) {
 struct Exchange {
   float4 (*slots)[2][kMaxCluster];  // [2][2][kMaxCluster]
   float4 (*warps)[2];               // [kThreads / 32][2]
-  int n, rank, turn;
-  // over(a, b, w): both values reduced over the first w lanes; b only if `two`
+  int n, wide, rank, turn;          // wide: n or the next power of two
+  // over(a, b, w): both values reduced over the first w lanes (a power of two); b only if `two`.  On entry to the last
+  // reduction, lanes without a CTA hold none_a and none_b, which change nothing.
   template <typename WARP>
-  CB_DEVICE void reduce(float4& a, float4& b, bool two, WARP over) {
+  CB_DEVICE void reduce(float4& a, float4& b, bool two, const float4 none_a, const float4 none_b, WARP over) {
     const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
     over(a, b, 32);
     if (lane == 0) {
@@ -55,9 +59,10 @@ struct Exchange {
     }
     if (n == 1) __syncthreads();
     else cluster_sync();
-    a = slots[t][0][lane & (n - 1)];
-    if (two) b = slots[t][1][lane & (n - 1)];
-    if (n > 1) over(a, b, n);
+    const int at = lane & (wide - 1);
+    a = at < n ? slots[t][0][at] : none_a;
+    if (two) b = at < n ? slots[t][1][at] : none_b;
+    if (n > 1) over(a, b, wide);
   }
   // the better of (x, i) and (ox, oi): larger value, lower index among equals (index -1: none)
   CB_DEVICE static void take(float& x, float& i, float ox, float oi) {
@@ -66,7 +71,8 @@ struct Exchange {
   }
   // a: two rows' (maximum, sum of 2^((l - maximum) k)); b (greedy): their (maximum, its lowest index)
   CB_DEVICE void stat2(float4& a, float4& b, bool greedy, float k) {
-    reduce(a, b, greedy, [&](float4& v, float4& y, int w) {
+    const float none = __int_as_float(-1);
+    reduce(a, b, greedy, make_float4(-INFINITY, 0.f, -INFINITY, 0.f), make_float4(-INFINITY, none, -INFINITY, none), [&](float4& v, float4& y, int w) {
       float m = v.x, n = v.z;
       for (int o = w >> 1; o; o >>= 1) {
         m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
@@ -91,13 +97,14 @@ struct Exchange {
   }
   // maxima of the scores .x and .z and their lowest indices .y, .w
   CB_DEVICE float4 best2(float4 a) {
-    float4 none = a;
-    reduce(a, none, false, [](float4& v, float4&, int w) { best(v, w); });
+    float4 unused = a;
+    const float none = __int_as_float(-1);
+    reduce(a, unused, false, make_float4(0.f, none, 0.f, none), a, [](float4& v, float4&, int w) { best(v, w); });
     return a;
   }
   CB_DEVICE float sum(float x) {
-    float4 a = make_float4(x, 0.f, 0.f, 0.f), none = a;
-    reduce(a, none, false, [](float4& v, float4&, int w) {
+    float4 a = make_float4(x, 0.f, 0.f, 0.f), unused = a;
+    reduce(a, unused, false, make_float4(0.f, 0.f, 0.f, 0.f), a, [](float4& v, float4&, int w) {
       for (int o = w >> 1; o; o >>= 1) v.x += __shfl_xor_sync(~0u, v.x, o);
     });
     return a.x;
@@ -105,12 +112,13 @@ struct Exchange {
 };
 
 // One cluster per request: its CTAs share the vocabulary.  A visited node costs one pass over its logits (while requests
-// are too few to fill HBM, a pass takes the node's first child along: most are accepted, and then need none); a rejection
+// are too few to fill HBM, or rows too short, a pass takes the node's first child along: most are accepted, and then need
+// none; 20.2 -> 14.7 us for 62 chains of 18 over 688 tokens); a rejection
 // of a token drawn from a distribution one pass over logits and distribution for the remainder's sum (not needed for
 // the last child, whose remainder goes straight into the draw); the end one pass over logits, distribution and noise.
 // What bounds it: the walk is a chain of passes, each a round of loads and one exchange (about 0.8 us), and with many
-// requests the rows' bytes.  One chain of 6 over 129,280 tokens 8.7 us on the device, 32 trees of 12 with distributions
-// 38 us (about 100 MB, 2.7 TB/s: requests whose walk is short leave the device idle), 61 of 16 over 32,003 bf16 22 us.
+// requests the rows' bytes.  One chain of 6 over 129,280 tokens 9.0 us on the device, 32 trees of 12 with distributions
+// 39 us (about 100 MB, 2.7 TB/s: requests whose walk is short leave the device idle), 61 of 16 over 32,003 bf16 21.5 us.
 // Asking L2 for the next rows ahead of the passes was slower (38 -> 46 us), a pass that takes the first child along is
 // faster (52 -> 45 us over three sets of trees).
 template <bool BF16, bool DRAFT>
@@ -126,7 +134,7 @@ __global__ void __launch_bounds__(kThreads, 2) tree_verify_kernel(
   __shared__ float4 s_stat;                            // of the first child: maximum, sum, index of the maximum
   const int n_cta = gridDim.x / clusters;
   const int rank = n_cta == 1 ? 0 : int(cluster_ctarank()), b = blockIdx.x / n_cta;
-  Exchange ex{sh_slots, sh_warps, n_cta, rank, 0};
+  Exchange ex{sh_slots, sh_warps, n_cta, n_cta > 1 ? 1 << (32 - __clz(n_cta - 1)) : 1, rank, 0};
   const int t0 = cu[b], n = cu[b + 1] - t0;
   for (int i = threadIdx.x; i < N; i += kThreads) {
     if (rank == 0) {
@@ -174,7 +182,7 @@ __global__ void __launch_bounds__(kThreads, 2) tree_verify_kernel(
     if (v == known) {
       st = s_stat;
     } else {
-      const int w = n_cta > 1 ? s_child[v] : -1;       // taken along
+      const int w = n_cta > 1 || V < 2 * kShare ? s_child[v] : -1;       // taken along
       const char* roww = w >= 0 ? row_of(w) : rowp;
       // the children's logits and draft probabilities, read while the pass runs
       if (int(threadIdx.x) < n) {
@@ -187,13 +195,12 @@ __global__ void __launch_bounds__(kThreads, 2) tree_verify_kernel(
       }
       float m[2] = {-INFINITY, -INFINITY}, s[2] = {0.f, 0.f};
       int best[2] = {-1, -1};
-      auto fold = [&](int r, const float* x, int cnt, int i0) {
+      auto fold = [&](int r, const float* x, int cnt, auto token) {     // token(u): x[u]'s
         float top = m[r];
         if (greedy) {
-          if (best[r] < 0) best[r] = i0;
 #pragma unroll
           for (int u = 0; u < kWide; ++u)
-            if (u < cnt && x[u] > top) { top = x[u]; best[r] = i0 + u * kThreads; }
+            if (u < cnt && x[u] > top) { top = x[u]; best[r] = token(u); }
         } else {
 #pragma unroll
           for (int u = 0; u < kWide; ++u)
@@ -206,12 +213,61 @@ __global__ void __launch_bounds__(kThreads, 2) tree_verify_kernel(
           if (u < cnt) s[r] += ex2v((x[u] - ref) * k);
         m[r] = top;
       };
-      if (w < 0) {                                     // sixteen loads in flight
+      if (BF16 && per >= kThreads * 8) {
+        // Eight tokens a load, on the row's own 16-byte grid (an odd length starts rows anywhere); the pieces at the ends
+        // of the CTA's share are put together from single tokens.  Twice the bytes in flight: 48.6 -> 40.2 us for 83
+        // chains of 11 greedy over 32,568 tokens.  Shares under a piece a thread leave threads idle and were slower
+        // (25.9 -> 28.0 us at 2,700 tokens a CTA), and fp32 gains nothing from its four a load.
+        auto piece = [&](const char* row, int i) -> uint4 {
+          const uint16_t* h = reinterpret_cast<const uint16_t*>(row);
+          if (i >= lo && i + 8 <= hi) return *reinterpret_cast<const uint4*>(h + i);
+          uint32_t x[4];
+#pragma unroll
+          for (int t = 0; t < 4; ++t) {
+            const int a = i + 2 * t;
+            x[t] = (a >= lo && a < hi ? h[a] : 0xff80u) | (a + 1 >= lo && a + 1 < hi ? h[a + 1] : 0xff80u) << 16;
+          }
+          return make_uint4(x[0], x[1], x[2], x[3]);
+        };
+        auto first = [&](const char* row) {             // this thread's first piece
+          const int off = int(reinterpret_cast<uintptr_t>(row + int64_t(lo) * 2) & 15) / 2;
+          return lo - off + int(threadIdx.x) * 8;
+        };
+        auto add = [&](int r, const uint4& p, const uint4& q, int i0) {
+          const uint32_t word[8] = {p.x, p.y, p.z, p.w, q.x, q.y, q.z, q.w};
+          float x[16];
+#pragma unroll
+          for (int t = 0; t < 16; ++t) x[t] = __uint_as_float(t & 1 ? word[t / 2] & 0xffff0000u : word[t / 2] << 16);
+          fold(r, x, 16, [&](int t) { return i0 + t + t / 8 * (kThreads - 1) * 8; });
+        };
+        const uint4 none = make_uint4(0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u);      // -inf
+        constexpr int STEP = kThreads * 8;
+        if (w < 0) {
+          for (int i0 = first(rowp); i0 < hi; i0 += 4 * STEP) {
+            uint4 x[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) x[u] = i0 + u * STEP < hi ? piece(rowp, i0 + u * STEP) : none;
+            add(0, x[0], x[1], i0);
+            add(0, x[2], x[3], i0 + 2 * STEP);
+          }
+        } else {
+          for (int i0 = first(rowp), i1 = first(roww); i0 < hi || i1 < hi; i0 += 2 * STEP, i1 += 2 * STEP) {
+            uint4 x[4];
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+              x[u] = i0 + u * STEP < hi ? piece(rowp, i0 + u * STEP) : none;
+              x[2 + u] = i1 + u * STEP < hi ? piece(roww, i1 + u * STEP) : none;
+            }
+            add(0, x[0], x[1], i0);
+            add(1, x[2], x[3], i1);
+          }
+        }
+      } else if (w < 0) {                              // sixteen loads in flight
         for (int i0 = lo + int(threadIdx.x); i0 < hi; i0 += kThreads * kWide) {
           float x[kWide];
 #pragma unroll
           for (int u = 0; u < kWide; ++u) x[u] = i0 + u * kThreads < hi ? logit(i0 + u * kThreads) : -INFINITY;
-          fold(0, x, kWide, i0);
+          fold(0, x, kWide, [&](int u) { return i0 + u * kThreads; });
         }
       } else {
         for (int i0 = lo + int(threadIdx.x); i0 < hi; i0 += kThreads * kUnroll) {
@@ -222,8 +278,9 @@ __global__ void __launch_bounds__(kThreads, 2) tree_verify_kernel(
             x[u] = i < hi ? logit(i) : -INFINITY;
             y[u] = i < hi ? at(roww, i) : -INFINITY;
           }
-          fold(0, x, kUnroll, i0);
-          fold(1, y, kUnroll, i0);
+          auto token = [&](int u) { return i0 + u * kThreads; };
+          fold(0, x, kUnroll, token);
+          fold(1, y, kUnroll, token);
         }
       }
       float4 both = make_float4(m[0], s[0], m[1], s[1]);
@@ -392,6 +449,29 @@ __global__ void __launch_bounds__(256) tree_commit_kernel(const int64_t* __restr
     }
 }
 
+// Clusters of c CTAs that the device holds at once: a property of device and kernel, asked once.
+template <typename F>
+cudaError_t clusters_that_fit(F f, int variant, int c, int* fit) {
+  constexpr int kDevices = 16;
+  static std::atomic<int> known[kDevices][4][kMaxCluster + 1];           // 1 + clusters
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev < kDevices && (*fit = known[dev][variant][c].load() - 1) >= 0) return cudaSuccess;
+  if (c > 8 && (e = cudaFuncSetAttribute(f, cudaFuncAttributeNonPortableClusterSizeAllowed, 1)) != cudaSuccess) return e;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = c; attr.val.clusterDim.y = 1; attr.val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(c);
+  cfg.blockDim = dim3(kThreads);
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  if ((e = cudaOccupancyMaxActiveClusters(fit, f, &cfg)) != cudaSuccess) return e;
+  if (dev < kDevices) known[dev][variant][c].store(*fit + 1);
+  return cudaSuccess;
+}
+
 }  // namespace tree
 
 cudaError_t tree_verify(const void* logits, bool bf16, int64_t ld, int V, const int* tokens, const int* cu,
@@ -401,14 +481,17 @@ cudaError_t tree_verify(const void* logits, bool bf16, int64_t ld, int V, const 
   if (B == 0) return cudaSuccess;
   auto f = bf16 ? (draft ? tree::tree_verify_kernel<true, true> : tree::tree_verify_kernel<true, false>)
                 : (draft ? tree::tree_verify_kernel<false, true> : tree::tree_verify_kernel<false, false>);
-  // CTAs per request: as many as keep all requests on the device at once (two CTAs per SM), each with a thousand
-  // tokens or more
-  int dev = 0, sms = 0;
-  cudaError_t e = cudaGetDevice(&dev);
-  if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-  if (e != cudaSuccess) return e;
-  int c = 1;
-  while (c < tree::kMaxCluster && int64_t(B) * c * 2 <= 2 * sms && V / (2 * c) >= 1024) c *= 2;
+  // CTAs per request: as many as keep all requests on the device at once (two CTAs per SM, a cluster within one GPC),
+  // each with kShare tokens or more.  16 chains over 129,280 tokens take 20.9 us with 16 CTAs each, which do not all
+  // fit, 18.0 with 13; 86 over 10,260 tokens 13.7 with 2, 12.5 with 3.
+  int c = std::max(1, std::min(tree::kMaxCluster, V / tree::kShare));
+  cudaError_t e = cudaSuccess;
+  while (c > 1) {
+    int fit = 0;
+    if ((e = tree::clusters_that_fit(f, (bf16 ? 2 : 0) + (draft ? 1 : 0), c, &fit)) != cudaSuccess) return e;
+    if (B <= fit) break;
+    --c;
+  }
   if (c > 8 && (e = cudaFuncSetAttribute(f, cudaFuncAttributeNonPortableClusterSizeAllowed, 1)) != cudaSuccess) return e;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;

@@ -271,6 +271,31 @@ def test_tree_verify_many_requests():
     assert 0 < int((v.n_accepted > 0).sum()) < 150
 
 
+@pytest.mark.parametrize("requests,V,probs,dtype", [
+    (16, 20011, False, torch.float32), (20, 32003, True, torch.bfloat16), (48, 20500, False, torch.bfloat16),
+    (86, 4100, True, torch.float32), (70, 700, False, torch.float32), (70, 700, False, torch.bfloat16)])
+def test_tree_verify_shares_of_the_vocabulary(requests, V, probs, dtype):
+    """Numbers of CTAs per request that are no powers of two, shares that end inside a 16-byte piece, short rows."""
+    parents = [tree(1 + i % 6, i, chain=i % 2 == 0) for i in range(requests)]
+    check_verify(parents, verify_inputs(parents, V, requests, probs, dtype, temps=(0.8, 0.0)))
+
+
+def test_tree_verify_unaligned_bf16_rows():
+    """bf16 logits that start at an odd column of a wider tensor whose other columns hold NaN."""
+    parents = [tree(6, i, chain=True) for i in range(3)]
+    kw = verify_inputs(parents, 70001, 4, False, torch.bfloat16, temps=(0.9, 0.0, 1.0))
+    plan, _ = make_plan(parents, [0] * 3)
+    on = {k: x.to(DEV) if x is not None else None for k, x in kw.items()}
+    a = spec.tree_verify(plan=plan, **on)
+    for first in (1, 2, 7):
+        wide = torch.full((18, 70011), float("nan"), device=DEV, dtype=torch.bfloat16)
+        wide[:, first:first + 70001] = on["logits"]
+        b = spec.tree_verify(plan=plan, **{**on, "logits": wide[:, first:first + 70001]})
+        assert torch.equal(a.path, b.path) and torch.equal(a.tokens, b.tokens)
+        # the rows' pieces start elsewhere, so sums round differently: 2e-5 as against 64 bits
+        torch.testing.assert_close(a.logprobs, b.logprobs, rtol=0, atol=2e-5)
+
+
 def test_tree_verify_duplicate_and_unknown_tokens():
     """Siblings with the same token, and tokens outside the vocabulary (never accepted), without draft probabilities."""
     parents = [[-1, 0, 0, 0, 0]] * 8
