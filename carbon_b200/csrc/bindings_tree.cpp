@@ -251,6 +251,7 @@ std::tuple<int, Tensor, Tensor, Tensor, Tensor> tree_verify(const Tensor& logits
                                 ptr<int>(parent), int(B), int(N), ptr<float>(uniforms), ptr<float>(noise),
                                 ptr<float>(temperature), ptr<float>(draft), o, o + B * N, o + B * (N + 1),
                                 reinterpret_cast<float*>(o + B * (2 * N + 1)), stream());
+  at::AutoDispatchBelowADInplaceOrView plain;           // views of a fresh tensor: nothing for autograd to note
   return {e, out.as_strided({B, N}, {N, 1}, 0), out.as_strided({B}, {1}, B * N),
           out.as_strided({B, N}, {N, 1}, B * (N + 1)), out.view(at::kFloat).as_strided({B, N}, {N, 1}, B * (2 * N + 1))};
 }
