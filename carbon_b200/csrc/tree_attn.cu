@@ -390,15 +390,16 @@ __global__ void __launch_bounds__(THREADS, 1) tree_mla_kernel(const __grid_const
     // the CTA's own half of the two tiles, lanes 16-23 and 24-31 of the peer's (past the end: the last row's).
     // Four lookups in turn wait for the page table four times: 129 against 125 us for 36 trees of 51 nodes and 128 heads
     // after 2 keys, 24.6 against 23.8 for 4 of 8 nodes after 1,000 fp8 keys.
-    auto rows_in = [&](const TreeItem& t, int j) -> int {
-      if (by_tma(t, t.tile + min(j + 1, t.n_tiles - 1))) return 0;      // then neither is fed
+    auto find = [&](const TreeItem& t, int j, int& off) -> int {          // page and offset in it
+      if (F8 && by_tma(t, t.tile + min(j + 1, t.n_tiles - 1))) return 0;  // then neither is fed
       const int half = rank ^ int(lane >> 4);
       const int pos = min((t.tile + j + int(lane >> 3 & 1)) * KT + half * 64 + r0 + int(lane & 7), t.ctx + t.n - 1);
-      return p.lay.table[size_t(t.b) * p.lay.P + pos / p.lay.page] * p.lay.page + pos % p.lay.page;
+      off = pos % p.lay.page;
+      return p.lay.table[size_t(t.b) * p.lay.P + pos / p.lay.page];
     };
     auto at = [&](int rows, int r) { return p.kv + int64_t(__shfl_sync(~0u, rows, r)) * RB; };
     TreeItem nx = p.work.items[i0];                     // items are read one ahead
-    int now = rows_in(nx, 0);
+    int off = 0, page = find(nx, 0, off), now = page * p.lay.page + off;
     pdl_wait();
     for (int i = i0; ok && i < i1; ++i) {
       const TreeItem it = nx;
@@ -412,7 +413,20 @@ __global__ void __launch_bounds__(THREADS, 1) tree_mla_kernel(const __grid_const
         const TreeItem& an = more ? it : nx;
         const int aj = more ? j + 2 : 0;
         const bool any = more || i + 1 < i1;
-        const int next = any ? rows_in(an, aj) : 0;
+        // fp8: looked up here; bf16: after the first tile's keys, when the next item has been read (for 36 trees of 51
+        // nodes x 128 heads after 2 keys 117.7 against 121.0 us; 100,000 fp8 keys take 55.4 that way and 53.4 this way)
+        int next = 0;
+        if (F8 && any) {
+          page = find(an, aj, off);
+          next = page * p.lay.page + off;
+        }
+        auto ahead = [&](int u) {                       // L2 prefetch two tiles on
+          if (!any || aj + u >= an.n_tiles || by_tma(an, an.tile + aj + u)) return;
+          const uint8_t* row = p.kv + int64_t(__shfl_sync(~0u, next, 8 * u + (lane >> 2))) * RB;
+#pragma unroll
+          for (int o = 0; o < RB; o += 512)
+            if (o + int(lane & 3) * 128 < RB) asm volatile("prefetch.global.L2 [%0];" ::"l"(row + o + (lane & 3) * 128));
+        };
         for (int u = 0; ok && u < m; ++u) {
           const int s = (g + u) & 1, ph = ((g + u) >> 1) & 1, tile = it.tile + j + u;
           uint8_t* st = sK + s * STAGE;
@@ -504,12 +518,15 @@ __global__ void __launch_bounds__(THREADS, 1) tree_mla_kernel(const __grid_const
           }
           __syncwarp();
           if (lane == 0) mbar_arrive_cluster(mapa_shared(smem_u32(&kfull[s]), 0));
-          if (fed && any && aj + u < an.n_tiles && !by_tma(an, an.tile + aj + u)) {      // L2 prefetch two tiles on
-            const uint8_t* row = p.kv + int64_t(__shfl_sync(~0u, next, 8 * u + (lane >> 2))) * RB;
-#pragma unroll
-            for (int o = 0; o < RB; o += 512)
-              if (o + int(lane & 3) * 128 < RB) asm volatile("prefetch.global.L2 [%0];" ::"l"(row + o + (lane & 3) * 128));
+          if constexpr (F8) {
+            if (fed) ahead(u);
+          } else if (u == 0 && any) {
+            page = find(an, aj, off);                   // not waited for before the second tile's keys
           }
+        }
+        if constexpr (!F8) {
+          next = page * p.lay.page + off;
+          for (int u = 0; u < m; ++u) ahead(u);
         }
         for (int u = 0; ok && u < m; ++u) {
           const int s = (g + u) & 1, ph = ((g + u) >> 1) & 1, tile = it.tile + j + u;
