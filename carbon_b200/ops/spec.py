@@ -212,8 +212,8 @@ def tree_mla(q: torch.Tensor, kv: torch.Tensor, plan: TreePlan, scale: float, d_
             # Whole key tiles that TMA cannot take from the cache as they lie (fp8 rows, small pages) are fed by the
             # kernel's warps (4.0 us a tile and CTA pair), or expanded to dense rows first (2.0 us a tile then, and
             # 2.8 us of every pair's time per staged tile; a launch): worth it from two row tiles per key tile and a
-            # few tiles per pair on.  32 requests near 4096, 6 nodes of 128 heads: 216 us fed, 152 us staged; one
-            # node: 70 us fed, 96 us staged; 4 requests of 500, 8 nodes: 23.8 us fed, 25.0 us staged.
+            # few tiles per pair on.  32 requests near 4096, 6 nodes of 128 heads: 204 us fed, 148 us staged; one
+            # node: 62 us fed, 85 us staged; 1 request of 700, 6 nodes: 19.3 us fed, 25.0 us staged.
             staged = None
             if (f8 or plan.page_size % 64) and tiles and work >= 2 * tiles and work >= 4 * plan._counts[0]:
                 staged = torch.empty(tiles * 128 * D, dtype=want, device=q.device)
