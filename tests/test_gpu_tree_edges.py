@@ -1,0 +1,110 @@
+"""Tree-speculation kernels at the edges of their arguments' ranges, against the definitions in 64 bits."""
+import pytest
+import torch
+
+from test_gpu_tree import DEV, check_verify, make_plan
+from carbon_b200.ops import spec
+
+pytestmark = pytest.mark.gpu
+LAST = 1 - 2.0 ** -24                                                       # the largest fp32 below 1
+
+
+# ----------------------------------------------------------------------------------------------------------------------
+# verification: what is left after a rejection
+# ----------------------------------------------------------------------------------------------------------------------
+def drafted_rows(B, kids, V, seed, dtype, filler):
+    """B requests, a root with ``kids`` children whose tokens are spread over the vocabulary; every other token of the
+    root's row has the logit ``filler``."""
+    g = torch.Generator().manual_seed(seed)
+    n = kids + 1
+    logits = torch.randn(B, n, V, generator=g)
+    logits[:, 0] = filler
+    tok = torch.zeros(B, n, dtype=torch.int32)
+    for b in range(B):
+        tok[b, 1:] = torch.randperm(V, generator=g)[:kids].int()
+        logits[b, 0, tok[b, 1:].long()] = torch.rand(kids, generator=g) * 4 - 2
+    kw = dict(logits=logits.view(B * n, V).to(dtype), tokens=tok.view(-1), uniforms=torch.zeros(B, n),
+              noise=torch.empty(B, V).exponential_(generator=g), temperature=torch.full((B,), 0.8), draft_probs=None)
+    return [[-1] + [0] * kids] * B, kw
+
+
+@pytest.mark.parametrize("V", [3, 500, 9000, 70001])
+@pytest.mark.parametrize("kids", [2, 3])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_tree_verify_drafts_hold_all_the_mass(V, kids, dtype):
+    """Only the drafted tokens are allowed: after the others are rejected the last one has probability 1 and is
+    accepted at every number below 1."""
+    parents, kw = drafted_rows(40, kids, V, V + kids, dtype, float("-inf"))
+    kw["uniforms"][:, 1:] = LAST
+    kw["uniforms"] = kw["uniforms"].view(-1)
+    v = check_verify(parents, kw)
+    assert bool((v.n_accepted == 1).all()) and bool((v.path[:, 1] == kids).all())
+
+
+def test_tree_verify_two_allowed_tokens():
+    lg = torch.full((3, 500), float("-inf"))
+    lg[0, 0], lg[0, 1] = -1.4074705, -2.530843
+    lg[1:, 7] = 0
+    for V in (2, 500):
+        lv = lg[:, :V].clone()
+        lv[1:, 0] = 0
+        v = check_verify([[-1, 0, 0]], dict(logits=lv, tokens=torch.tensor([0, 0, 1], dtype=torch.int32),
+                                            uniforms=torch.tensor([0, 0.9, LAST]), noise=torch.ones(1, V),
+                                            temperature=torch.tensor([0.8]), draft_probs=None))
+        assert v.path[0, :2].tolist() == [0, 2]
+
+
+@pytest.mark.parametrize("V", [500, 70001])
+def test_tree_verify_remainder_of_a_peaked_row(V):
+    """The first child holds all but 1e-3 to 1e-5 of the mass; the second is tested against what is left.  Its share
+    x / (sum of the rest) has the rounding of exponents up to 20 (20 * 2^-22 = 5e-6) and of the sum (1e-6): numbers
+    2e-5 below and above the 64-bit share are accepted and rejected."""
+    B = 40
+    for sign, taken in ((-1, 1), (1, 0)):
+        parents, kw = drafted_rows(B, 2, V, V, torch.float32, -8.0)
+        rows = kw["logits"].view(B, 3, V)
+        g = torch.Generator().manual_seed(V)
+        for b in range(B):
+            a, x = kw["tokens"][3 * b + 1:3 * b + 3].long().tolist()
+            rest = torch.rand((), generator=g).item() * 3
+            rows[b, 0, x] = torch.log(torch.tensor(float(V))) * 0.8 - 8.0 + rest
+            rows[b, 0, a] = rows[b, 0].div(0.8).logsumexp(0) * 0.8 + 0.8 * (7 + 4 * torch.rand((), generator=g).item())
+            p = (rows[b, 0].double() / 0.8).softmax(0)
+            p[a] = 0
+            kw["uniforms"][b, 1] = LAST
+            kw["uniforms"][b, 2] = (p[x] / p.sum()).item() * (1 + sign * 2e-5)
+        kw["uniforms"] = kw["uniforms"].view(-1)
+        v = check_verify(parents, kw)
+        assert bool((v.n_accepted == taken).all())
+
+
+def test_tree_verify_wide_roots_and_repeated_tokens():
+    """63 children of one node, some with the same token, with certain proposals: drawn numbers and numbers near 1."""
+    g = torch.Generator().manual_seed(11)
+    for V, top in ((40, 1.0), (3000, LAST)):
+        parents, kw = drafted_rows(12, 40 if V == 40 else 63, V, V, torch.float32, -3.0)
+        n = len(parents[0])
+        tok = kw["tokens"].view(12, n)
+        tok[:, 5::3] = tok[:, 4:5]                                          # repeats of node 4's token
+        kw["uniforms"] = (torch.rand(12 * n, generator=g) * top).clamp(max=LAST)
+        check_verify(parents, kw)
+
+
+def test_tree_verify_a_first_child_whose_own_drafts_hold_the_mass():
+    """The same two levels down: the accepted first child's row, whose sums may come with its parent's."""
+    B = 32
+    for V in (60, 900, 30000):
+        g = torch.Generator().manual_seed(V)
+        parents = [[-1, 0, 1, 1]] * B
+        logits = torch.full((B, 4, V), float("-inf"))
+        tok = torch.zeros(B, 4, dtype=torch.int32)
+        for b in range(B):
+            tok[b, 1:] = torch.randperm(V, generator=g)[:3].int()
+            logits[b, 0, tok[b, 1].long()] = 1.0
+            logits[b, 1, tok[b, 2:].long()] = torch.rand(2, generator=g) * 4 - 2
+            logits[b, 2:, 1] = 0.5
+        u = torch.tensor([0.0, LAST, LAST, LAST]).repeat(B)
+        v = check_verify(parents, dict(logits=logits.view(-1, V), tokens=tok.view(-1), uniforms=u,
+                                       noise=torch.empty(B, V).exponential_(generator=g),
+                                       temperature=torch.full((B,), 0.8), draft_probs=None))
+        assert bool((v.path[:, :3] == torch.tensor([0, 1, 3])).all())
