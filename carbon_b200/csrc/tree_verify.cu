@@ -9,6 +9,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <cfloat>
 
 namespace cb {
 namespace tree {
@@ -120,10 +121,10 @@ struct Exchange {
 // of a token drawn from a distribution one pass over logits and distribution for the remainder's sum (not needed for
 // the last child, whose remainder goes straight into the draw); the end one pass over logits, distribution and noise.
 // A certain proposal's rejection takes its token out.  While a quarter of the row is left its mass is a difference (whose
-// relative error is at most four times the sum's, about that of the exponentials).  Less may be far smaller than what was taken, and a child that is nearly all
-// of what is left may be all of it, with a probability of exactly 1: then it is a sum, the children still in and, from one
-// more pass over the logits (once a node), the tokens that no child has.  That pass at every node with a rejection took 61
-// trees of 16 over 20,000 tokens from 18.2 to 20.9 us, this rule to 19.0.
+// relative error is at most four times the sum's, about that of the exponentials).  Less may be far smaller than what
+// was taken, and a child that is nearly all of what is left may be all of it, with a probability of exactly 1: then it is
+// a sum, the children still in and, from one more pass over the logits (once a node), the tokens that no child has.  That
+// pass at every node with a rejection took 61 trees of 16 over 20,000 tokens from 18.2 to 20.9 us, this rule to 19.0.
 // What bounds it: the walk is a chain of passes, each a round of loads and one exchange (about 0.8 us), and with many
 // requests the rows' bytes.  One chain of 6 over 129,280 tokens 9.0 us on the device, 32 trees of 12 with distributions
 // 39 us (about 100 MB, 2.7 TB/s: requests whose walk is short leave the device idle), 61 of 16 over 32,003 bf16 21.5 us.
@@ -177,7 +178,8 @@ __global__ void __launch_bounds__(kThreads, 2) tree_verify_kernel(
   }
   __syncthreads();
   const bool greedy = !(T > 0.f);
-  const float k = greedy ? kLog2e : kLog2e / T;        // p = 2^((l - max) k) / total
+  // p = 2^((l - max) k) / total; k neither 0 (an infinite T: equal weights, and -inf stays out) nor infinite (a subnormal T)
+  const float k = greedy ? kLog2e : fminf(fmaxf(kLog2e / T, __int_as_float(1)), FLT_MAX);
   const int per = (V + n_cta - 1) / n_cta, lo = rank * per, hi = min(V, lo + per);
   const float* e = noise + size_t(b) * V;
   auto row_of = [&](int node) {

@@ -2,8 +2,7 @@
 import pytest
 import torch
 
-from test_gpu_tree import DEV, check_verify, make_plan
-from carbon_b200.ops import spec
+from test_gpu_tree import check_verify, tree, verify_inputs
 
 pytestmark = pytest.mark.gpu
 LAST = 1 - 2.0 ** -24                                                       # the largest fp32 below 1
@@ -108,3 +107,12 @@ def test_tree_verify_a_first_child_whose_own_drafts_hold_the_mass():
                                        noise=torch.empty(B, V).exponential_(generator=g),
                                        temperature=torch.full((B,), 0.8), draft_probs=None))
         assert bool((v.path[:, :3] == torch.tensor([0, 1, 3])).all())
+
+
+@pytest.mark.parametrize("heat", [float("inf"), 3e38, 1e-30, 1e-40])
+@pytest.mark.parametrize("probs", [False, True])
+def test_tree_verify_extreme_temperatures(heat, probs):
+    """Every positive temperature has a distribution: uniform where it is infinite, the maximum as it goes to zero (1e-40
+    is subnormal in fp32)."""
+    parents = [tree(5, i) for i in range(6)]
+    check_verify(parents, verify_inputs(parents, 3000, 21, probs, temps=(heat,)))
