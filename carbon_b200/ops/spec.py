@@ -305,7 +305,7 @@ def tree_verify(logits: torch.Tensor, tokens: torch.Tensor, plan: TreePlan, unif
 
 class CacheRows:
     """The caches whose rows move together: tensors [S, ...] (one row per slot, any row size that is a multiple of 4
-    bytes), contiguous and on one device.  Holds the tensors and, on a GPU, the table of their addresses."""
+    bytes), contiguous, on one device and starting on a 4-byte boundary.  Holds the tensors and, on a GPU, the table of their addresses."""
 
     def __init__(self, caches: Sequence[torch.Tensor]):
         self.caches = [c for c in caches if c is not None]
@@ -320,6 +320,8 @@ class CacheRows:
             if c.device != first.device or not c.is_contiguous() or nbytes % 4 or not nbytes:
                 raise ValueError("CacheRows: caches must be contiguous, on one device and have rows of a multiple of "
                                  "4 bytes")
+            if c.data_ptr() % 4:
+                raise ValueError("CacheRows: caches must start on a 4-byte boundary")
             rows += [c.data_ptr(), nbytes]
         self.max_row = max(rows[1::2])
         self.wide = all(x % 16 == 0 for x in rows)
