@@ -171,6 +171,12 @@ def _need(what: str, t: torch.Tensor, dev: int, dtype) -> None:
                          f"{'' if t.is_contiguous() else ' (not contiguous)'}")
 
 
+def _aligned(what: str, t: torch.Tensor) -> None:
+    """Rows are read 16 bytes at a time (row sizes are multiples of 16): an address off that grid would fault."""
+    if t.data_ptr() % 16:
+        raise ValueError(f"{what} must start on a 16-byte boundary (address modulo 16: {t.data_ptr() % 16})")
+
+
 def _launched(code: int, what: str) -> None:
     if code:
         raise RuntimeError(f"{what}: CUDA error {code} at launch")
@@ -180,7 +186,8 @@ def tree_mla(q: torch.Tensor, kv: torch.Tensor, plan: TreePlan, scale: float, d_
              sink: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Attention of the plan's nodes over the paged latent cache: q [T, H, D], kv [S, D] bf16 (or the fp8 cache rows,
     uint8 [S, row_bytes], with q in fp16; q is converted), D = 576 (MLA) or 512 (latent MQA) -> [T, H, 512] bf16.
-    sink [H]: per-head attention-sink logit.  A node that sees no key gives zeros."""
+    On a GPU kv is contiguous and starts on a 16-byte boundary.  sink [H]: per-head attention-sink logit.  A node that
+    sees no key gives zeros."""
     T, H, D = q.shape
     f8 = kv.dtype == torch.uint8
     if T != plan.T:
@@ -202,8 +209,11 @@ def tree_mla(q: torch.Tensor, kv: torch.Tensor, plan: TreePlan, scale: float, d_
         _need("tree_mla: kv", kv, dev, torch.uint8 if f8 else torch.bfloat16)
         if kv.dim() != 2 or kv.shape[1] != (_ROW_BYTES[D] if f8 else D):
             raise ValueError(f"tree_mla: kv of shape {tuple(kv.shape)} does not hold rows for width {D}")
+        _aligned("tree_mla: kv", kv)
         want = torch.float16 if f8 else torch.bfloat16
         qk = q if q.dtype is want and q.is_contiguous() else q.to(want).contiguous()
+        if qk.data_ptr() % 16:                           # the tensor map needs it
+            qk = qk.clone()
         if sink is not None:
             _need("tree_mla: sink", sink, dev, torch.float32)
         out = torch.empty(T, H, 512, dtype=torch.bfloat16, device=q.device)

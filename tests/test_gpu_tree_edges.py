@@ -2,7 +2,8 @@
 import pytest
 import torch
 
-from test_gpu_tree import check_verify, tree, verify_inputs
+from test_gpu_tree import DEV, SCALE, check_verify, inputs, make_plan, tree, verify_inputs
+from carbon_b200.ops import spec
 
 pytestmark = pytest.mark.gpu
 LAST = 1 - 2.0 ** -24                                                       # the largest fp32 below 1
@@ -116,3 +117,23 @@ def test_tree_verify_extreme_temperatures(heat, probs):
     is subnormal in fp32)."""
     parents = [tree(5, i) for i in range(6)]
     check_verify(parents, verify_inputs(parents, 3000, 21, probs, temps=(heat,)))
+
+
+# ----------------------------------------------------------------------------------------------------------------------
+# attention: where rows begin
+# ----------------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("f8,page", [(False, 64), (False, 24), (True, 64)])
+def test_tree_mla_rows_off_a_16_byte_boundary(f8, page):
+    """A cache that starts off a 16-byte boundary is refused on the host; queries that do are copied."""
+    plan, S = make_plan([tree(6, 0)], [300], page, 16)
+    q, kv, _ = inputs(plan, S, 16, 576, f8, seed=3)
+    want = spec.tree_mla(q, kv, plan, SCALE)
+    for off in (1, 4) if f8 else (1, 2, 4):
+        flat = torch.empty(kv.numel() + 16, dtype=kv.dtype, device=DEV)
+        moved = flat[off:off + kv.numel()].view(kv.shape)
+        with pytest.raises(ValueError, match="16-byte boundary"):
+            spec.tree_mla(q, moved, plan, SCALE)
+        flat = torch.empty(q.numel() + 16, dtype=q.dtype, device=DEV)
+        moved = flat[off:off + q.numel()].view(q.shape)
+        moved.copy_(q)
+        assert torch.equal(spec.tree_mla(moved, kv, plan, SCALE), want)

@@ -19,3 +19,16 @@ def test_cache_rows_refuse_an_address_between_words():
                 spec.CacheRows([torch.zeros(16, 4), view])
         else:
             spec.CacheRows([view])
+
+
+@pytest.mark.parametrize("dtype", [torch.uint8, torch.bfloat16])
+def test_rows_off_a_16_byte_boundary_are_refused(dtype):
+    """What tree_mla asks of its cache before a launch (the row kernels read 16 bytes at a time)."""
+    flat = torch.zeros(656 * 4 + 16, dtype=dtype)
+    for off in range(0, 17):
+        rows = flat[off:off + 656 * 4].view(4, 656)
+        if rows.data_ptr() % 16:
+            with pytest.raises(ValueError, match="16-byte boundary"):
+                spec._aligned("tree_mla: kv", rows)
+        else:
+            spec._aligned("tree_mla: kv", rows)
