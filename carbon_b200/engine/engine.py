@@ -596,7 +596,11 @@ class Engine:
                 c = self.cache
                 self._cache_rows = spec.CacheRows(c.latent + c.index_k + ([c.tok] if c.tok is not None else []))
             spec.tree_commit(self._cache_rows, plan, got.path, got.n_accepted)
-        counts, tokens = got.n_accepted.tolist(), got.tokens.tolist()
+        # one copy: the attention's status word, and nothing of a step whose attention gave up is handed on
+        B = len(reqs)
+        words = torch.cat([plan.status, got.n_accepted, got.tokens.flatten()]).tolist()
+        plan.check(words[0])
+        counts, tokens = words[1:1 + B], [words[1 + B + b * plan.N:1 + B + (b + 1) * plan.N] for b in range(B)]
         accepted = []
         for r, (toks, _), a, new in zip(reqs, trees, counts, tokens):
             if new[a] < 0:

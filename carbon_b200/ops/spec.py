@@ -142,10 +142,11 @@ class TreePlan:
         at = self._at + 2 * self.B + 1 + 2 * self.T
         return self._host[at:at + self.T].tolist()
 
-    def check(self) -> None:
-        """Raise if a kernel of this plan gave up a wait (reads from the device)."""
-        if int(self.status):
-            raise RuntimeError(f"tree_mla: device status {int(self.status)}: a bounded wait ran out")
+    def check(self, status: Optional[int] = None) -> None:
+        """Raise if a kernel of this plan gave up a wait.  Reads ``status`` from the device unless the caller has."""
+        code = int(self.status) if status is None else status
+        if code:
+            raise RuntimeError(f"tree_mla: device status {code}: a bounded wait ran out")
 
     def slots(self, b: int, n: Optional[int] = None) -> List[int]:
         """Cache slots of request b's first n positions (default: its context and all its nodes)."""

@@ -2,7 +2,11 @@
 import pytest
 import torch
 
+from carbon_b200.config import tiny_config
+from carbon_b200.engine.engine import Engine
+from carbon_b200.models.weights import WeightSource
 from carbon_b200.ops import spec
+from carbon_b200.ref.model import init_weights
 
 
 def test_cache_rows_refuse_an_address_between_words():
@@ -32,3 +36,37 @@ def test_rows_off_a_16_byte_boundary_are_refused(dtype):
                 spec._aligned("tree_mla: kv", rows)
         else:
             spec._aligned("tree_mla: kv", rows)
+
+
+# ----------------------------------------------------------------------------------------------------------------------
+# the engine's step: failures
+# ----------------------------------------------------------------------------------------------------------------------
+def two_requests():
+    cfg = tiny_config().replace(index_n_heads=0, index_topk=0)
+    eng = Engine(cfg, "cpu", source=WeightSource(cfg, state=init_weights(cfg, seed=0)), num_pages=64, page_size=16)
+    reqs = [eng.add_request([1, 2, 3]), eng.add_request([4, 5, 6, 7])]
+    eng.prefill(reqs)
+    return eng, reqs, [([5, 8, 9], [-1, 0, 0]), ([6, 3], [-1, 0])]
+
+
+def state(reqs):
+    return [(list(r.out), r.n_cached, r.seq_len) for r in reqs]
+
+
+def test_a_wait_that_ran_out_fails_the_step():
+    """The attention's status word (set here by hand, in the middle of the forward) ends the step with an error, and no
+    request has grown."""
+    eng, reqs, trees = two_requests()
+    forward, before = eng.model.forward, state(reqs)
+
+    def give_up(fb, cache):
+        logits = forward(fb, cache)
+        fb.tree.status.fill_(3)
+        return logits
+
+    eng.model.forward = give_up
+    with pytest.raises(RuntimeError, match="status 3"):
+        eng.verify_tree(reqs, trees)
+    assert state(reqs) == before
+    eng.model.forward = forward
+    assert all(len(o) >= 1 for o in eng.verify_tree(reqs, trees))           # the next step starts with a clean word
