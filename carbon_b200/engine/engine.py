@@ -562,7 +562,8 @@ class Engine:
         context and its own branch; ``tree_verify`` walks down each tree, and the accepted branch's cache rows move
         behind the context.  temperature: one number or one per request (0: greedy).  draft_probs [all nodes, V]: the
         distribution each node's children were drawn from; without it drafts are certain proposals.  With temperature
-        the emitted tokens are distributed as the target's own samples.  Returns the new tokens per request (>= 1)."""
+        the emitted tokens are distributed as the target's own samples.  Returns the new tokens per request (>= 1); where
+        it raises, no request has grown."""
         from ..ops import spec
 
         if self.model.pctx.world > 1:
@@ -601,10 +602,11 @@ class Engine:
         words = torch.cat([plan.status, got.n_accepted, got.tokens.flatten()]).tolist()
         plan.check(words[0])
         counts, tokens = words[1:1 + B], [words[1 + B + b * plan.N:1 + B + (b + 1) * plan.N] for b in range(B)]
-        accepted = []
-        for r, (toks, _), a, new in zip(reqs, trees, counts, tokens):
+        for r, a, new in zip(reqs, counts, tokens):              # before any request grows
             if new[a] < 0:
                 raise RuntimeError(f"request {r.rid}: the target's logits leave no token (not finite)")
+        accepted = []
+        for r, (toks, _), a, new in zip(reqs, trees, counts, tokens):
             r.out += [int(toks[0])] + new[:a]                # tokens whose KV is now valid in the cache
             r.n_cached = r.seq_len
             accepted.append(new[:a + 1])

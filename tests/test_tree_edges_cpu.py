@@ -70,3 +70,24 @@ def test_a_wait_that_ran_out_fails_the_step():
     assert state(reqs) == before
     eng.model.forward = forward
     assert all(len(o) >= 1 for o in eng.verify_tree(reqs, trees))           # the next step starts with a clean word
+
+
+def test_one_request_without_a_token_leaves_all_unchanged():
+    """The second of two requests has no finite logits: the step raises, neither request has grown, and the step can be
+    run again."""
+    eng, reqs, trees = two_requests()
+    forward, before = eng.model.forward, state(reqs)
+
+    def spoil(fb, cache):
+        logits = forward(fb, cache).clone()
+        logits[3:] = float("nan")
+        return logits
+
+    eng.model.forward = spoil
+    with pytest.raises(RuntimeError, match=f"request {reqs[1].rid}"):
+        eng.verify_tree(reqs, trees)
+    assert state(reqs) == before
+    eng.model.forward = forward
+    other, theirs, _ = two_requests()
+    assert eng.verify_tree(reqs, trees) == other.verify_tree(theirs, trees)
+    assert state(reqs) == state(theirs)
