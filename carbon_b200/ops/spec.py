@@ -27,6 +27,7 @@ from ..ref import ops as R
 from ._ext import ext
 
 _ROW_BYTES = {576: 656, 512: 528}      # an fp8 cache row (ref.ops.latent_fp8_row_bytes)
+_STAGE_BYTES = 512 << 20               # of the dense rows of one call: 465,000 keys of 576 dims
 MAX_NODES = 64           # nodes of one request's tree: one bit each in a node's mask
 
 
@@ -183,6 +184,22 @@ def _launched(code: int, what: str) -> None:
         raise RuntimeError(f"{what}: CUDA error {code} at launch")
 
 
+def _stage_rows(counts: Sequence[int], f8: bool, page_size: int, D: int) -> int:
+    """Dense rows that a call expands its whole key tiles to before the attention (0: it does not).
+
+    Whole key tiles that TMA cannot take from the cache as they lie (fp8 rows, small pages) are fed by the kernel's warps
+    (4.0 us a tile and CTA pair), or expanded to dense rows first (2.0 us a tile then, and 2.8 us of every pair's time per
+    staged tile; a launch): worth it from two row tiles per key tile and a few tiles per pair on.  32 requests near 4096,
+    6 nodes of 128 heads: 204 us fed, 148 us staged; one node: 62 us fed, 85 us staged; 1 request of 700, 6 nodes: 19.3 us
+    fed, 25.0 us staged.  Not past _STAGE_BYTES of dense rows: they are 1.76 times the fp8 cache rows, once per request even
+    of pages that requests share, in the middle of a step on a device whose cache may fill it (fed past it: 1.25 times the
+    time at 128 requests of 4096 keys and 6 nodes, 1.4 times with 24 nodes)."""
+    pairs, tiles, work = counts[0], counts[4], counts[5]
+    if not (f8 or page_size % 64) or not tiles or work < 2 * tiles or work < 4 * pairs:
+        return 0
+    return tiles * 128 if tiles * 128 * D * 2 <= _STAGE_BYTES else 0
+
+
 def tree_mla(q: torch.Tensor, kv: torch.Tensor, plan: TreePlan, scale: float, d_latent: int = 512,
              sink: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Attention of the plan's nodes over the paged latent cache: q [T, H, D], kv [S, D] bf16 (or the fp8 cache rows,
@@ -219,15 +236,9 @@ def tree_mla(q: torch.Tensor, kv: torch.Tensor, plan: TreePlan, scale: float, d_
             _need("tree_mla: sink", sink, dev, torch.float32)
         out = torch.empty(T, H, 512, dtype=torch.bfloat16, device=q.device)
         if T:
-            parts, tiles, work = plan._counts[3:6]
-            # Whole key tiles that TMA cannot take from the cache as they lie (fp8 rows, small pages) are fed by the
-            # kernel's warps (4.0 us a tile and CTA pair), or expanded to dense rows first (2.0 us a tile then, and
-            # 2.8 us of every pair's time per staged tile; a launch): worth it from two row tiles per key tile and a
-            # few tiles per pair on.  32 requests near 4096, 6 nodes of 128 heads: 204 us fed, 148 us staged; one
-            # node: 62 us fed, 85 us staged; 1 request of 700, 6 nodes: 19.3 us fed, 25.0 us staged.
-            staged = None
-            if (f8 or plan.page_size % 64) and tiles and work >= 2 * tiles and work >= 4 * plan._counts[0]:
-                staged = torch.empty(tiles * 128 * D, dtype=want, device=q.device)
+            parts = plan._counts[3]
+            rows = _stage_rows(plan._counts, f8, plan.page_size, D)
+            staged = torch.empty(rows * D, dtype=want, device=q.device) if rows else None
             buf = torch.empty(parts * 128 * 514, dtype=torch.float32, device=q.device) if parts else None
             _launched(ext().tree_mla(qk, kv, plan.cu, plan.ctx, plan.table, plan.mask, plan.page_size, plan._work,
                                      plan._counts, buf, staged, float(scale), sink, plan.status, out), "tree_mla")

@@ -91,3 +91,35 @@ def test_one_request_without_a_token_leaves_all_unchanged():
     other, theirs, _ = two_requests()
     assert eng.verify_tree(reqs, trees) == other.verify_tree(theirs, trees)
     assert state(reqs) == state(theirs)
+
+
+# ----------------------------------------------------------------------------------------------------------------------
+# which calls expand their rows first
+# ----------------------------------------------------------------------------------------------------------------------
+def counts_of(requests, ctx, nodes, heads=128, page=64):
+    """The counts of a plan whose requests share their pages."""
+    from carbon_b200.ops._ext import available, ext
+
+    if not available():
+        pytest.skip("the extension is not built")
+    table = list(range(-(-(ctx + nodes) // page)))
+    code, _, counts, _ = ext().tree_plan([table] * requests, [ctx] * requests, [[-1] + [0] * (nodes - 1)] * requests, page,
+                                         heads, 74)
+    assert code == 0
+    return counts
+
+
+def test_expanded_rows_are_bounded():
+    """A batch of fp8 requests expands its whole key tiles; one whose dense rows would pass the limit is fed instead, and
+    so is what the rule never expands."""
+    c = counts_of(32, 4096, 6)
+    assert spec._stage_rows(c, True, 64, 576) == 32 * 4096 and spec._stage_rows(c, True, 64, 512) == 32 * 4096
+    assert spec._stage_rows(c, False, 24, 576) == 32 * 4096
+    assert spec._stage_rows(c, False, 64, 576) == 0                          # TMA takes them as they lie
+    assert spec._stage_rows(counts_of(32, 4096, 1), True, 64, 576) == 0      # one row tile per key tile
+    assert spec._stage_rows(counts_of(1, 700, 6), True, 64, 576) == 0        # few tiles
+    for requests in (32, 64):                                                # 4.8 and 9.7 GB of dense rows
+        assert spec._stage_rows(counts_of(requests, 131072, 6), True, 64, 576) == 0
+    most = spec._STAGE_BYTES // (576 * 2 * 128)
+    ok, over = counts_of(1, most * 128, 6), counts_of(1, (most + 1) * 128, 6)
+    assert spec._stage_rows(ok, True, 64, 576) == most * 128 and spec._stage_rows(over, True, 64, 576) == 0
