@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from test_gpu_tree import DEV, SCALE, check_verify, inputs, make_plan, tree, verify_inputs
+from test_gpu_tree import DEV, SCALE, check_verify, close, exact, inputs, make_plan, tree, verify_inputs
 from carbon_b200.ops import spec
 
 pytestmark = pytest.mark.gpu
@@ -137,3 +137,57 @@ def test_tree_mla_rows_off_a_16_byte_boundary(f8, page):
         moved = flat[off:off + q.numel()].view(q.shape)
         moved.copy_(q)
         assert torch.equal(spec.tree_mla(moved, kv, plan, SCALE), want)
+
+
+# ----------------------------------------------------------------------------------------------------------------------
+# attention over rows that are expanded to dense tiles first
+# ----------------------------------------------------------------------------------------------------------------------
+STAGED = [
+    # contexts (nodes 6, the fourth request has none), heads, width, fp8, page, sink
+    ([1501, 1280, 127, 900, 1999, 128, 1407, 1153, 640, 1663, 1282, 1700], 128, 576, True, 64, False),
+    ([1501, 1280, 127, 900, 1999, 128, 1407, 1153, 640, 1663, 1282, 1700], 128, 512, True, 64, True),
+    ([1501, 1280, 127, 900, 1999, 128, 1407, 1153, 640, 1663, 1282, 1700], 128, 576, False, 24, True),
+    ([1501, 1280, 127, 900, 1999, 128, 1407, 1153, 640, 1663, 1282, 1700], 128, 512, False, 5, False),
+    ([1501, 1280, 127, 900, 1999, 128, 1407, 1153, 640, 1663, 1282, 1700], 128, 576, True, 7, True),
+    ([9000], 128, 576, True, 64, False),
+]
+
+
+def staged_plan(ctx, H, page, nodes=6):
+    n = [0 if b == 3 else nodes for b in range(len(ctx))]
+    return make_plan([tree(k, i) if k else [] for i, k in enumerate(n)], ctx, page, H)
+
+
+@pytest.mark.parametrize("ctx,H,D,f8,page,sink", STAGED)
+def test_tree_mla_expanded_rows(ctx, H, D, f8, page, sink):
+    plan, S = staged_plan(ctx, H, page, 33 if len(ctx) == 1 else 6)
+    assert spec._stage_rows(plan._counts, f8, page, D) == 128 * sum(c // 128 for b, c in enumerate(ctx) if b != 3)
+    q, kv, sk = inputs(plan, S, H, D, f8, seed=D + page, sink=sink)
+    close(spec.tree_mla(q, kv, plan, SCALE, sink=sk), exact(q, kv, plan, SCALE, sk))
+
+
+@pytest.mark.parametrize("D,page,f8", [(576, 64, True), (512, 64, True), (576, 24, False), (512, 5, False)])
+def test_tree_mla_expanded_rows_garbage_outside_the_mask(D, page, f8):
+    """Unwritten rows and nodes of other branches that hold NaN and infinities do not reach a node that does not see
+    them."""
+    ctx = [1501, 1280, 127, 900, 1999, 128, 1407, 1153, 640, 1663, 1282, 1700]
+    masks = [[(1 << i) | 1 for i in range(6)] if b != 3 else [] for b in range(12)]     # the root and itself
+    plan, S = make_plan([tree(6, b) if b != 3 else [] for b in range(12)], ctx, page, 128, masks=masks)
+    assert spec._stage_rows(plan._counts, f8, page, D)
+    q, kv, _ = inputs(plan, S, 128, D, f8, seed=31)
+    want = exact(q, kv, plan, SCALE)
+    live = torch.zeros(S, dtype=torch.bool, device=DEV)
+    rows, at = [], 0
+    for b in range(12):
+        slots = torch.tensor(plan.slots(b), device=DEV, dtype=torch.long)
+        live[slots] = True
+        if b != 3:
+            live[slots[ctx[b] + 4]] = False                                 # node 4 of every tree: seen by itself alone
+            rows += [at + i for i in (0, 1, 2, 3, 5)]
+            at += 6
+    kv[~live] = 0x7F if f8 else float("nan")
+    if not f8:
+        kv[~live, ::2] = float("inf")
+    got = spec.tree_mla(q, kv, plan, SCALE)
+    close(got[rows], want[rows])
+    assert bool(torch.isnan(got[4::6]).all())
