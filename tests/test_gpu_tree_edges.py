@@ -2,7 +2,8 @@
 import pytest
 import torch
 
-from test_gpu_tree import DEV, SCALE, check_verify, close, exact, inputs, make_plan, tree, verify_inputs
+from test_gpu_tree import (DEV, SCALE, check_verify, close, engine_cfg, exact, inputs, make_plan, rows_of, tree,
+                           verify_inputs)
 from carbon_b200.ops import spec
 
 pytestmark = pytest.mark.gpu
@@ -113,8 +114,8 @@ def test_tree_verify_a_first_child_whose_own_drafts_hold_the_mass():
 @pytest.mark.parametrize("heat", [float("inf"), 3e38, 1e-30, 1e-40])
 @pytest.mark.parametrize("probs", [False, True])
 def test_tree_verify_extreme_temperatures(heat, probs):
-    """Every positive temperature has a distribution: uniform where it is infinite, the maximum as it goes to zero (1e-40
-    is subnormal in fp32)."""
+    """Every positive temperature has a distribution: uniform where it is infinite, the maximum as it goes to zero
+    (1e-40 is subnormal in fp32)."""
     parents = [tree(5, i) for i in range(6)]
     check_verify(parents, verify_inputs(parents, 3000, 21, probs, temps=(heat,)))
 
@@ -191,3 +192,120 @@ def test_tree_mla_expanded_rows_garbage_outside_the_mask(D, page, f8):
     got = spec.tree_mla(q, kv, plan, SCALE)
     close(got[rows], want[rows])
     assert bool(torch.isnan(got[4::6]).all())
+
+
+# ----------------------------------------------------------------------------------------------------------------------
+# the engine's step, row by row
+# ----------------------------------------------------------------------------------------------------------------------
+def dense_engine(kind, **kw):
+    """A model without routed experts: no router choice can flip between two ways of computing a row."""
+    from carbon_b200.engine.engine import Engine
+    from carbon_b200.models.weights import WeightSource
+    from carbon_b200.ref.model import init_weights
+
+    cfg = engine_cfg(kind)
+    cfg = cfg.replace(n_dense_layers=cfg.n_layers)
+    src = WeightSource(cfg, state=init_weights(cfg, seed=0))
+    return cfg, lambda: Engine(cfg, device="cuda", source=src, num_pages=96, page_size=64, **kw)
+
+
+@pytest.mark.parametrize("kind", ["dense", "dense_fp8", "latent"])
+def test_engine_attention_of_every_node_and_layer(kind, monkeypatch):
+    """The attention of every layer of a tree step, node by node, against the definition in 64 bits over the request's
+    pages: the context's rows and those of the node's own branch, found from the trees and the page tables alone."""
+    from carbon_b200.models import deepseek
+
+    cfg, make = dense_engine(kind)
+    g = torch.Generator().manual_seed(1)
+    ps = [torch.randint(0, cfg.vocab_size, (k,), generator=g).tolist() for k in (70, 131, 300)]
+    trees = [([5, 6, 7, 8], [-1, 0, 0, 1]), ([9], [-1]), ([1, 2, 3, 4, 5, 6], [-1, 0, 1, 1, 2, 0])]
+    eng = make()
+    reqs = [eng.add_request(p) for p in ps]
+    eng.prefill(reqs)
+    calls, plain = [], spec.tree_mla
+
+    def record(q, kv, plan, scale, r, sink=None):
+        out = plain(q, kv, plan, scale, r, sink=sink)
+        calls.append((q.double(), kv.clone(), scale, sink, out.clone()))
+        return out
+
+    monkeypatch.setattr(deepseek.S, "tree_mla", record)
+    eng.verify_tree(reqs, trees)
+    assert len(calls) == cfg.n_layers
+    for q, kv, scale, sink, out in calls:
+        t = 0
+        for req, p, (toks, par) in zip(reqs, ps, trees):
+            for i in range(len(toks)):
+                branch, k = [], i
+                while k >= 0:
+                    branch.insert(0, k)
+                    k = par[k]
+                at = list(range(len(p))) + [len(p) + k for k in branch]
+                slots = torch.tensor([req.pages[x // 64] * 64 + x % 64 for x in at], device=DEV)
+                keys = rows_of(kv[slots], q.shape[2]).double()
+                s = q[t] @ keys.t() * scale
+                if sink is not None:
+                    s = torch.cat([s, sink.double()[:, None]], 1)
+                close(out[t], torch.softmax(s, 1)[:, :len(at)] @ keys[:, :512])
+                t += 1
+        assert t == q.shape[0]
+
+
+@pytest.mark.parametrize("kind", ["dense", "dense_fp8", "latent", "dsa"])
+def test_engine_every_node_is_nearest_its_own_branch(kind):
+    """The logits of every node of a tree step against all the nodes' branches run as decode rows: its own is the
+    nearest.  (How far is not asserted: roundings that differ move a row by some percent through the fp8 products.)"""
+    cfg, make = dense_engine(kind)
+    g = torch.Generator().manual_seed(1)
+    ps = [torch.randint(0, cfg.vocab_size, (k,), generator=g).tolist() for k in (70, 131, 300)]
+    trees = [([5, 6, 7, 8], [-1, 0, 0, 1]), ([9], [-1]), ([1, 2, 3, 4, 5, 6], [-1, 0, 1, 1, 2, 0])]
+    eng, rows = make(), []
+    for p, (toks, par) in zip(ps, trees):
+        for i in range(len(toks)):
+            branch, k = [], i
+            while k >= 0:
+                branch.insert(0, toks[k])
+                k = par[k]
+            r = eng.add_request(p)
+            eng.prefill([r])
+            for t in branch:
+                lg = eng.decode([r], [t])
+            rows.append(lg[0].float())
+            eng.release(r)
+    reqs = [eng.add_request(p) for p in ps]
+    eng.prefill(reqs)
+    seen = {}
+    forward = eng.model.forward
+
+    def keep(fb, cache):
+        seen["logits"] = forward(fb, cache).clone()
+        return seen["logits"]
+
+    eng.model.forward = keep
+    eng.verify_tree(reqs, trees)
+    want = torch.stack(rows)
+    assert torch.cdist(seen["logits"].float(), want).argmin(1).tolist() == list(range(len(want)))
+
+
+@pytest.mark.parametrize("kind", ["dense", "dense_fp8", "latent", "dsa"])
+def test_engine_greedy_trees_follow_the_target(kind):
+    """Greedy trees from prompt lookup and from the target itself: replayed token by token through plain decoding, every
+    emitted token is the target's best but for rounding.  The GPU model's logits are within 12 % of the oracle's norm,
+    0.12 rms a logit; three standard deviations of the difference of two are 0.12 * sqrt(2) * 3 = 0.5 rms."""
+    from carbon_b200.engine.spec import ModelDrafter, NgramDrafter
+
+    cfg, make = dense_engine(kind)
+    g = torch.Generator().manual_seed(2)
+    base = torch.randint(0, cfg.vocab_size, (20,), generator=g).tolist()
+    ps = [base * 3, torch.randint(0, cfg.vocab_size, (280,), generator=g).tolist()]
+    for drafter in (NgramDrafter(), ModelDrafter(make())):
+        outs = make().generate_speculative(ps, 10, drafter, n_draft=6, tree=True)
+        eng = make()
+        reqs = [eng.add_request(p) for p in ps]
+        logits = eng.prefill(reqs).float()
+        for i in range(10):
+            tok = [o[i] for o in outs]
+            short = logits.amax(-1) - logits[torch.arange(2), tok]
+            assert bool((short <= 0.5 * logits.pow(2).mean(-1).sqrt()).all()), (i, short)
+            if i < 9:
+                logits = eng.decode(reqs, tok).float()
