@@ -496,9 +496,10 @@ def tree_verify(logits: torch.Tensor, tokens, parents, uniforms, noise: torch.Te
     when u_c q(x_c) < r(x_c), q the distribution its token was drawn from (draft_probs[v]; without them the token is
     a certain proposal, q = 1 at it); a rejection leaves r <- max(r - q, 0) renormalised (r itself if nothing is
     left).  Where no child is accepted the next token is argmax_i r_i / noise_i (noise ~ Exp(1): a draw from r; ties
-    to the lowest index).  T <= 0: r is one at the lowest-index maximum of the logits and no noise is used.
-    Returns (path, tokens, logprobs): the accepted nodes from the root, the emitted tokens (-1 if r has no mass) and
-    their log-probabilities under softmax(logits / T) (T = 1 when greedy)."""
+    to the lowest index).  A child whose token is outside the vocabulary is passed over.  T <= 0: r is one at the
+    lowest-index maximum of the logits and no noise is used.  Returns (path, tokens, logprobs): the accepted nodes from
+    the root, the emitted tokens (-1 if r has no mass) and their log-probabilities under softmax(logits / T) (T = 1 when
+    greedy)."""
     heat = temperature if temperature > 0 else 1.0
     v, path, toks, lps = 0, [0], [], []
     while True:
@@ -514,6 +515,8 @@ def tree_verify(logits: torch.Tensor, tokens, parents, uniforms, noise: torch.Te
         nxt = -1
         for c in [j for j in range(len(parents)) if parents[j] == v]:
             x = int(tokens[c])
+            if not 0 <= x < r.shape[0]:
+                continue
             q = torch.zeros_like(r)
             if draft_probs is None:
                 q[x] = 1.0

@@ -123,3 +123,21 @@ def test_expanded_rows_are_bounded():
     most = spec._STAGE_BYTES // (576 * 2 * 128)
     ok, over = counts_of(1, most * 128, 6), counts_of(1, (most + 1) * 128, 6)
     assert spec._stage_rows(ok, True, 64, 576) == most * 128 and spec._stage_rows(over, True, 64, 576) == 0
+
+
+# ----------------------------------------------------------------------------------------------------------------------
+# verification: tokens that are not in the vocabulary
+# ----------------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("temperature", [0.0, 1.0])
+@pytest.mark.parametrize("probs", [False, True])
+def test_tokens_outside_the_vocabulary_are_never_accepted(temperature, probs):
+    """-1 and -5 would be the row's own last entries, 6 and 2^31 - 1 are past its end: none is accepted or changes what
+    is left, and a sibling inside the vocabulary is tested as if alone."""
+    logits = torch.tensor([[0.0, 1.0, 2.0, 3.0, 4.0, 9.0]]).repeat(7, 1)
+    tokens = torch.tensor([0, -1, -5, 6, 2 ** 31 - 1, -2 ** 31, 5], dtype=torch.int32)
+    for last in (5, -1):
+        tokens[6] = last
+        plan = spec.TreePlan([[0, 1]], [0], [[-1] + [0] * 6], 4, device="cpu")
+        v = spec.tree_verify(logits, tokens, plan, torch.zeros(7), torch.ones(1, 6), torch.tensor([temperature]),
+                             torch.full((7, 6), 1 / 6) if probs else None)
+        assert v.n_accepted.tolist() == [int(last == 5)] and v.tokens[0, 0].item() == 5
