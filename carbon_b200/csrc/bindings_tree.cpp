@@ -41,7 +41,7 @@ cb::TreeLayout layout(const Tensor& cu, const Tensor& ctx, const Tensor& table, 
 // tiles, key tiles over all items and the most partial results of a row tile
 std::tuple<Tensor, std::vector<int64_t>> tree_schedule(const std::vector<int64_t>& n, const std::vector<int64_t>& ctx,
                                                        int64_t H, int64_t clusters) {
-  constexpr int64_t kTile = 128, kOver = 2, kPiece = 1;
+  constexpr int64_t kTile = 128, kOver = 2;
   constexpr double kMerge = 1.5, kPart = 0.04;
   const int64_t B = int64_t(n.size());
   std::vector<int64_t> cu(B + 1, 0);
@@ -72,9 +72,8 @@ std::tuple<Tensor, std::vector<int64_t>> tree_schedule(const std::vector<int64_t
         const Load ld = heap.top();
         heap.pop();
         const int64_t rest = r.tiles - at, room = share - ld.first - kOver;
-        if (!force && room < std::min(rest, kPiece)) return false;
-        // a remainder shorter than a piece stays here
-        const int64_t take = force || rest < room + std::min(kPiece, share / 16 + 1) ? rest : room;
+        if (!force && room < 1) return false;
+        const int64_t take = force ? rest : std::min(rest, room);    // a remainder of one tile goes on, too
         auto& list = lists[ld.second];
         pieces.push_back({ld.second, list.size()});
         list.push_back({int(r.b), int(r.row), int(at), int(take), -1, int(ctx[r.b]), int(cu[r.b]), int(n[r.b])});
@@ -88,7 +87,7 @@ std::tuple<Tensor, std::vector<int64_t>> tree_schedule(const std::vector<int64_t
     }
     return true;
   };
-  const int64_t even = std::max((total + clusters - 1) / clusters, kPiece + kOver);
+  const int64_t even = std::max((total + clusters - 1) / clusters, 1 + kOver);
   double least = 0;
   int64_t take = -1;
   for (int64_t share = even, tries = 0; tries < 16; ++tries, share += std::max<int64_t>(1, even / 24)) {

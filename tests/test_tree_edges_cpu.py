@@ -141,3 +141,17 @@ def test_tokens_outside_the_vocabulary_are_never_accepted(temperature, probs):
         v = spec.tree_verify(logits, tokens, plan, torch.zeros(7), torch.ones(1, 6), torch.tensor([temperature]),
                              torch.full((7, 6), 1 / 6) if probs else None)
         assert v.n_accepted.tolist() == [int(last == 5)] and v.tokens[0, 0].item() == 5
+
+
+def test_schedule_sends_a_one_tile_remainder_on():
+    """27 and 10 key tiles over three pairs: at a share of 15 (13 tiles and 2 for an item's start and end) the first row
+    tile is cut twice, and the single tile that is left goes to the pair with the least work like any other piece."""
+    from carbon_b200.ops._ext import available, ext
+
+    if not available():
+        pytest.skip("the extension is not built")
+    ctx = [27 * 128 - 1, 10 * 128 - 1]
+    _, host, (used, items, *_), _ = ext().tree_plan([list(range(c // 64 + 1)) for c in ctx], ctx, [[-1], [-1]], 64, 16, 3)
+    w, head = host.tolist(), (used + 4) // 4 * 4
+    got = sorted(tuple(w[head + 8 * i + k] for k in (0, 2, 3)) for i in range(items))
+    assert used == 3 and got == [(0, 0, 13), (0, 13, 13), (0, 26, 1), (1, 0, 10)]
