@@ -634,10 +634,14 @@ class Engine:
                              tree: bool = False, temperature: float = 0.0, seed: int = 0):
         """Generation with draft-and-verify steps (``n_draft`` drafts + 1 row per request per step).  Greedy chains by
         default; ``tree``: drafted trees (the drafter's ``propose_tree``); temperature > 0: tokens sampled from the
-        target's distribution at that temperature (``verify_tree``; ``seed`` fixes the random numbers)."""
+        target's distribution at that temperature (``verify_tree``; ``seed`` fixes the random numbers).  Trees and sampled
+        chains take at most 63 drafts per step."""
+        from ..ops.spec import MAX_NODES
         from .spec import NgramDrafter
 
         drafter = drafter or NgramDrafter()
+        if tree or temperature > 0:
+            n_draft = min(n_draft, MAX_NODES - 1)
         reqs = [self.add_request(p) for p in prompts]
         logits = self.prefill(reqs)
         gen = None

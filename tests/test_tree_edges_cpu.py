@@ -155,3 +155,29 @@ def test_schedule_sends_a_one_tile_remainder_on():
     w, head = host.tolist(), (used + 4) // 4 * 4
     got = sorted(tuple(w[head + 8 * i + k] for k in (0, 2, 3)) for i in range(items))
     assert used == 3 and got == [(0, 0, 13), (0, 13, 13), (0, 26, 1), (1, 0, 10)]
+
+
+class Long:
+    """Drafts as many tokens as it is asked for: the known continuation, then zeros."""
+
+    def __init__(self, full):
+        self.full = full
+
+    def propose(self, tokens, n):
+        left = self.full[len(tokens):]
+        return (left + [0] * n)[:n]
+
+    def propose_tree(self, tokens, n):
+        return self.propose(tokens, n), list(range(n))
+
+
+@pytest.mark.parametrize("kw", [dict(tree=True), dict(temperature=1e-4), dict(tree=True, temperature=1e-4)])
+def test_more_drafts_than_a_tree_holds(kw):
+    """A drafter is asked for as many tokens as fit a tree (64 nodes with the pending one), however many the caller
+    allows."""
+    cfg = tiny_config().replace(index_n_heads=0, index_topk=0)
+    w = init_weights(cfg, seed=0)
+    make = lambda: Engine(cfg, "cpu", source=WeightSource(cfg, state=w), num_pages=64, page_size=16)
+    prompt = [1, 2, 3, 4]
+    ref = make().generate([prompt], 70)
+    assert make().generate_speculative([prompt], 70, Long(prompt + ref[0]), n_draft=200, **kw) == ref
