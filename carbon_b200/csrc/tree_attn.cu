@@ -9,9 +9,10 @@
 // which leaves room for two score tiles.  (One CTA with M = 128 rows would need all 512 columns for O.)
 //
 // Key tiles come into shared memory by TMA where they lie there as the tensor core reads them: whole tiles of bf16 rows
-// in pages of a multiple of 64.  fp8 rows, other pages and each request's last tiles (which end, or belong to the tree)
-// are fed by warps: global memory -> registers -> fp16 / bf16 in the swizzled layout.  tree_merge_kernel joins row tiles
-// whose keys were split over CTA pairs.
+// in pages of a multiple of 64, or rows that tree_stage_kernel has expanded to dense fp16 / bf16 first (fp8 rows and other
+// pages, in calls large enough to read them twice).  Else such rows, and each request's last tiles always (which end, or
+// belong to the tree), are fed by warps: global memory -> registers -> fp16 / bf16 in the swizzled layout.
+// tree_merge_kernel joins row tiles whose keys were split over CTA pairs.
 #include <cudaTypedefs.h>
 #include <cuda_fp16.h>
 #include "ptx.cuh"
@@ -175,12 +176,17 @@ __global__ void __launch_bounds__(256) tree_stage_kernel(const uint8_t* __restri
 // What bounds it: a 128-key tile is 128 x 128 x 1088 MACs, 2176 cycles of a pair's tensor cores; it takes 2.06 us with
 // the keys in L2 (1.28 PFLOP/s, 64 tiles on 74 pairs), 2.7 us with 32 tiles per pair from HBM.  The ring holds two
 // tiles (Q 72 KB, 2 x 72 KB of keys, P), so the matrix instructions of one tile cover the softmax of the other only
-// partly (tensor pipe 62 % active): its 1,600 cycles of latency are 60 loading and 180 for the maximum, 320 exchanging
+// partly (tensor pipe 66 % active): its 1,600 cycles of latency are 60 loading and 180 for the maximum, 320 exchanging
 // it, 660 exponentials (16 a cycle), 380 storing P and its proxy fence, and the barriers to and from the issuing thread
 // add 1,200.  Large calls run into the power cap first (1.57 GHz at 1.1 PFLOP/s).
 // ---------------------------------------------------------------------------------------------------------------
 // A fed row with a NaN or an infinity in a tile that holds tree rows: Q·K^T sees it (its scores are NaN, and so is every
 // node that sees it), but the values P·V multiplies by a weight of zero for the other branches' nodes are made zero.
+//
+// Arrives at the leader's barriers from the other CTA have the default scope, the CTA's.  What they announce stays in the
+// arriving warp's own SM: its shared memory (after the proxy fence) and TMEM, which that SM's tensor core reads when the
+// leader issues for the pair.  Nothing has to become visible to another SM first, and a release to the cluster's scope
+// before each arrive took 3.0 us a tile instead of 2.07.
 //
 // The tensor maps see a row as 64-dim atoms: (64 dims, rows, atoms), so one TMA load fills several chunks.
 struct Maps {

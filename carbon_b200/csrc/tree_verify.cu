@@ -126,8 +126,9 @@ struct Exchange {
 // a sum, the children still in and, from one more pass over the logits (once a node), the tokens that no child has.  That
 // pass at every node with a rejection took 61 trees of 16 over 20,000 tokens from 18.2 to 20.9 us, this rule to 19.0.
 // What bounds it: the walk is a chain of passes, each a round of loads and one exchange (about 0.8 us), and with many
-// requests the rows' bytes.  One chain of 6 over 129,280 tokens 9.0 us on the device, 32 trees of 12 with distributions
-// 39 us (about 100 MB, 2.7 TB/s: requests whose walk is short leave the device idle), 61 of 16 over 32,003 bf16 21.5 us.
+// requests the rows' bytes.  On the device, three sets of drafts each: one chain of 6 over 129,280 tokens 10.3 us, 32
+// trees of 12 with distributions 45 us (about 100 MB, 2.2 TB/s: requests whose walk is short leave the device idle), 61 of
+// 16 over 32,003 bf16 22.8 us.
 // Asking L2 for the next rows ahead of the passes was slower (38 -> 46 us), a pass that takes the first child along is
 // faster (52 -> 45 us over three sets of trees).
 template <bool BF16, bool DRAFT>
